@@ -16,6 +16,8 @@
 //   with sinks: l += exp(sink_h - m) at the end; sink_h is a learned logit of query head h that takes a share
 //   of the weight and carries no value (scale applies to the dot products only)
 // Values may have another width (value_dim) than keys and queries (head_dim).
+// row_stats, if given: float [token][query head], m + log(l) in units of log2 (infinity where nothing is visible), with which
+// 2^(s_j log2(e) - row_stats) is the weight of key j.
 // (reference: kernels/attention_kernel.py:184-251, :516-586).  Everything is float.
 #include "common.h"
 
@@ -28,7 +30,7 @@ __global__ __launch_bounds__(SIA_WAVE) void attention_generic_kernel(
     const int* __restrict__ block_table, int table_width, const int* __restrict__ seq_of_token,
     const int* __restrict__ positions, T* __restrict__ out, int n_heads, int n_kv, int head_dim,
     int value_dim, int page_size, float scale, int window, int chunk, const float* __restrict__ sinks, float cap,
-    int keep_first) {
+    int keep_first, float* __restrict__ row_stats) {
     __shared__ float q_s[ATTN_MAX_HEAD_DIM];
     __shared__ float p_s[SIA_WAVE];
     __shared__ int page_s[SIA_WAVE];
@@ -92,6 +94,7 @@ __global__ __launch_bounds__(SIA_WAVE) void attention_generic_kernel(
 
     T* o = out + ((size_t)n * n_heads + h) * value_dim;
     if (sinks) l += expf(sinks[h] - m);   // m is finite: a token always sees itself
+    if (row_stats && lane == 0) row_stats[(size_t)n * n_heads + h] = row_stat(m, l);
     const float inv = 1.f / l;
 #pragma unroll
     for (int dd = 0; dd < ATTN_MAX_HEAD_DIM / SIA_WAVE; ++dd) {
@@ -105,11 +108,11 @@ __global__ __launch_bounds__(SIA_WAVE) void attention_generic_kernel(
 SIA_EXPORT int sia_attention_max_head_dim() { return ATTN_MAX_WRITTEN_HEAD_DIM; }
 SIA_EXPORT int sia_attention_generic_max_head_dim() { return ATTN_MAX_HEAD_DIM; }
 
-SIA_EXPORT int sia_attention_generic(const void* q, int q_row_stride, const void* k_pages, const void* v_pages,
-                                     const int* block_table, int table_width, const int* seq_of_token,
-                                     const int* positions, void* out, int n_tokens, int n_heads, int n_kv,
-                                     int head_dim, int value_dim, int page_size, float scale, int window, int chunk,
-                                     const float* sinks, float cap, int keep_first, int dtype, hipStream_t stream) {
+static int launch_generic(const void* q, int q_row_stride, const void* k_pages, const void* v_pages,
+                          const int* block_table, int table_width, const int* seq_of_token,
+                          const int* positions, void* out, int n_tokens, int n_heads, int n_kv,
+                          int head_dim, int value_dim, int page_size, float scale, int window, int chunk,
+                          const float* sinks, float cap, int keep_first, float* row_stats, int dtype, hipStream_t stream) {
     if (n_tokens <= 0) return 0;
     if (head_dim <= 0 || head_dim > ATTN_MAX_HEAD_DIM || value_dim <= 0 || value_dim > ATTN_MAX_HEAD_DIM || n_kv <= 0 || n_heads % n_kv || page_size <= 0 ||
         n_heads > 65535 || cap < 0.f || keep_first < 0)
@@ -119,10 +122,31 @@ SIA_EXPORT int sia_attention_generic(const void* q, int q_row_stride, const void
     hipLaunchKernelGGL(attention_generic_kernel<T>, grid, block, 0, stream, (const T*)q, q_row_stride,         \
                        (const T*)k_pages, (const T*)v_pages, block_table, table_width, seq_of_token, positions, \
                        (T*)out, n_heads, n_kv, head_dim, value_dim, page_size, scale, window, chunk, sinks, cap, \
-                       keep_first)
+                       keep_first, row_stats)
     if (dtype == SIA_F32) LAUNCH(float);
     else if (dtype == SIA_BF16) LAUNCH(bf16_t);
     else return SIA_BAD_ARGUMENT;
 #undef LAUNCH
     return SIA_LAUNCH_CHECK();
+}
+
+SIA_EXPORT int sia_attention_generic(const void* q, int q_row_stride, const void* k_pages, const void* v_pages,
+                                     const int* block_table, int table_width, const int* seq_of_token,
+                                     const int* positions, void* out, int n_tokens, int n_heads, int n_kv,
+                                     int head_dim, int value_dim, int page_size, float scale, int window, int chunk,
+                                     const float* sinks, float cap, int keep_first, int dtype, hipStream_t stream) {
+    return launch_generic(q, q_row_stride, k_pages, v_pages, block_table, table_width, seq_of_token, positions, out, n_tokens,
+                          n_heads, n_kv, head_dim, value_dim, page_size, scale, window, chunk, sinks, cap, keep_first, nullptr,
+                          dtype, stream);
+}
+
+// The same without window, blocks, cap and kept positions, and the rows' statistics beside the result (float [n_tokens][n_heads]).
+SIA_EXPORT int sia_attention_generic_stats(const void* q, int q_row_stride, const void* k_pages, const void* v_pages,
+                                           const int* block_table, int table_width, const int* seq_of_token,
+                                           const int* positions, void* out, int n_tokens, int n_heads, int n_kv,
+                                           int head_dim, int value_dim, int page_size, float scale, const float* sinks,
+                                           float* row_stats, int dtype, hipStream_t stream) {
+    if (!row_stats) return SIA_BAD_ARGUMENT;
+    return launch_generic(q, q_row_stride, k_pages, v_pages, block_table, table_width, seq_of_token, positions, out, n_tokens,
+                          n_heads, n_kv, head_dim, value_dim, page_size, scale, 0, 0, sinks, 0.f, 0, row_stats, dtype, stream);
 }

@@ -109,6 +109,16 @@ _SIGNATURES = {
                           _c_ptr, _c_float, _c_int, _c_ptr],
     "sia_attention_max_head_dim": [],
     "sia_attention_generic_max_head_dim": [],
+    "sia_attention_generic_stats": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int,
+                                    _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_ptr, _c_int, _c_ptr],
+    "sia_weigh_plain": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
+                        _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_ptr],
+    "sia_rope_axes_max": [],
+    "sia_rope_axes_kv_write": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int,
+                               _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr],
+    "sia_evict_workspace": [_c_int] * 5,
+    "sia_evict": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                  _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr],
     "sia_gemm_generic": [_c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr],
     "sia_gemm_f32": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr],
     "sia_gemm_f32_workspace": [_c_ptr, _c_ptr, _c_int, _c_int, _c_int],
@@ -324,11 +334,13 @@ class HipKernels:
         self.core.sia_delta_rule_workspace.restype = ctypes.c_longlong
         self.core.sia_linear_unit_workspace.restype = ctypes.c_longlong
         self.core.sia_bonus_recurrence_workspace.restype = ctypes.c_longlong
+        self.core.sia_evict_workspace.restype = ctypes.c_longlong
         self.tiled_experts = True        # many slots in bfloat16: experts' products on the matrix cores, slots sorted by expert
         self._attn_libs = {}
         # the short way to the current stream's handle, where this torch has it (a few microseconds less a launch)
         self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self._device_index = torch.device(device).index or 0
+        self._own_device = torch.device("cuda", self._device_index)
         self.use_mfma_attention = True   # tests switch it off to reach the plain kernel in bfloat16
         self.use_skinny_gemm = True      # few-row bfloat16 products by this package's kernel, not the library
         self.fuse_norms = True           # few rows: residual add in the product before a norm, row scale in the one after
@@ -1676,6 +1688,54 @@ class HipKernels:
             n, n_heads, n_kv_written, head_dim, rotary_dim, page_size, _DT[qkv.dtype], self._stream()),
             "rope_kv_write")
 
+    def rope_axes_kv_write(self, qkv, n_heads, n_kv_written, head_dim, sections, cos, sin, rotary_positions, ctx, cache,
+                           order="blocks", pairing="half"):
+        """Rotation by positions with several axes, and the cache write.  ``qkv [tokens, (n_heads + 2 n_kv_written) head_dim]``: q
+        is rotated in place; k is rotated and, like v, written to place ``ctx.positions[t]`` of the token's sequence (what the
+        rows hold of k and v stays as it was).  ``rotary_positions``: int32 ``[axes, tokens]``, up to four axes; a place and the positions are
+        different things.  ``sections``: rotary pairs of each axis; twice their sum is the rotated part of a head.  ``order``: the pairs
+        are dealt to the axes in ``"blocks"`` (the first ``sections[0]`` to axis 0, and so on) or ``"cycled"`` (pair ``j`` to axis
+        ``j mod axes`` while that has fewer than its section, else to axis 0).  ``pairing``: ``"half"`` (elements ``i`` and ``i +
+        rotary_dim / 2``) or ``"interleaved"`` (neighbours).  ``cos``, ``sin``: float32 tables ``[positions, pairs]``; a position
+        outside them is taken at the nearest row."""
+        self._want(qkv, "qkv")
+        if qkv.dtype not in _DT or qkv.dim() != 2:
+            raise KernelError(f"qkv must be a float32 or bfloat16 matrix, is {qkv.dtype} {tuple(qkv.shape)}")
+        n, width = qkv.shape
+        if n_heads <= 0 or n_kv_written < 0 or head_dim <= 0 or width != (n_heads + 2 * n_kv_written) * head_dim:
+            raise KernelError(f"qkv row of {width} does not hold {n_heads} + 2*{n_kv_written} heads of {head_dim}")
+        if n != ctx.n_tokens:
+            raise KernelError(f"qkv has {n} rows, the step {ctx.n_tokens} tokens")
+        sections, most = tuple(int(c) for c in sections), self.core.sia_rope_axes_max()
+        axes, half = len(sections), sum(sections)
+        if not 0 < axes <= most or min(sections) < 0 or not 0 < 2 * half <= head_dim:
+            raise KernelError(f"sections {sections} are not pairs of 1 to {most} axes that a head of {head_dim} holds")
+        if order not in ("blocks", "cycled"):
+            raise KernelError(f"order must be 'blocks' or 'cycled', got {order!r}")
+        if order == "cycled" and any(c and axes * (c - 1) + a >= half for a, c in enumerate(sections) if a):
+            raise KernelError(f"sections {sections} cannot be dealt in turn: an axis behind the first would have more pairs than turns")
+        if pairing not in ("half", "interleaved"):
+            raise KernelError(f"pairing must be 'half' or 'interleaved', got {pairing!r}")
+        for t, what in ((cos, "cos table"), (sin, "sin table")):
+            self._want(t, what, torch.float32)
+            if t.dim() != 2 or t.shape[0] < 1 or t.shape[1] != half:
+                raise KernelError(f"{what} {tuple(t.shape)} does not hold {half} pairs")
+        if cos.shape != sin.shape:
+            raise KernelError(f"cos and sin tables differ: {tuple(cos.shape)} and {tuple(sin.shape)}")
+        self._want(rotary_positions, "rotary positions", torch.int32, (axes, n))
+        table = k_pages = v_pages = None
+        page_size = pages = 0
+        if n_kv_written:
+            k_pages, v_pages, table, page_size = cache.k_pages, cache.v_pages, cache.block_table, cache.page_size
+            self._check_pages(k_pages, v_pages, table, page_size, n_kv_written, head_dim, qkv.dtype, ctx)
+            pages = k_pages.shape[0]
+        self._same_device(qkv, cos, sin, rotary_positions, k_pages, v_pages, table)
+        self._check(self.core.sia_rope_axes_kv_write(
+            _ptr(qkv), width, _ptr(cos), _ptr(sin), cos.shape[0], _ptr(rotary_positions), (ctypes.c_int * most)(*sections), axes,
+            int(order == "cycled"), _ptr(ctx.positions), _ptr(ctx.seq_of_token), _ptr(table),
+            table.shape[1] if table is not None else 0, _ptr(k_pages), _ptr(v_pages), pages, n, n_heads, n_kv_written, head_dim, 2 * half,
+            int(pairing == "interleaved"), page_size, _DT[qkv.dtype], self._stream()), "rope_axes_kv_write")
+
     def qkv_to_cache(self, x, w_qkv, n_heads, n_kv_written, head_dim, rotary_dim, cos, sin, ctx, cache,
                      value_dim=None, bias=None, qk_norm=None, page_dim=None, q_temp=None, extra_columns=0,
                      values_are_keys=False, value_mix=None, give_values=False):
@@ -1962,6 +2022,96 @@ class HipKernels:
             n_kv_heads, head_dim, value_dim, page, float(scale), int(window or 0), int(chunk or 0), _ptr(sinks),
             float(softcap or 0.0), int(keep_first), _DT[qkv.dtype], self._stream()), "attention_generic")
         return out
+
+    def _same_device(self, *tensors):
+        """Raises for tensors that lie on another device than these kernels are launched on."""
+        for t in tensors:
+            if t is not None and t.device != self._own_device:
+                raise KernelError(f"a tensor lies on {t.device}, the kernels run on {self._own_device}")
+
+    def _check_weights(self, cache, ctx, n_kv):
+        """The sums that a cache keeps beside its keys: ``[slots, n_kv, places]``, room for every place of the step."""
+        weights, most = cache.weights, int(max(ctx.kv_bound or 0, ctx.max_kv_len))
+        if weights is None:
+            raise KernelError("the cache keeps no weights (LayerCache.weights)")
+        self._want(weights, "weights", torch.float32)
+        if weights.dim() != 3 or weights.shape[0] < 1 or weights.shape[1] != n_kv or weights.shape[2] < max(1, most):
+            raise KernelError(f"weights {tuple(weights.shape)} are not [slots, {n_kv}, places] with room for {most} places")
+        for t, what in ((ctx.state_slots, "state slots"), (ctx.kv_len, "lengths")):
+            self._want(t, what, torch.int32, (ctx.n_seqs,))
+        return weights, most
+
+    def weighed_attention(self, qkv, n_heads, n_kv_heads, head_dim, scale, ctx, cache, value_dim=None, sinks=None):
+        """``paged_attention`` (without window, blocks and cap) that also adds up how much weight every cached key gets:
+        ``cache.weights[slot, g, place]`` (float32 ``[slots, n_kv_heads, places]``; a sequence's row is ``ctx.state_slots[s]``, each
+        sequence with a row of its own) grows by the sum, over the sequence's tokens of this step and the query heads of ``g``, of
+        their softmax weights.  The sums of the places that the step itself has written begin at zero.  ``sinks`` take their share
+        of a row's weight and have no place.  Prompts, portions and single tokens, mixed as ``ctx`` says."""
+        self._want(qkv, "qkv")
+        if qkv.dtype not in _DT or qkv.dim() != 2:
+            raise KernelError(f"qkv must be a float32 or bfloat16 matrix, is {qkv.dtype} {tuple(qkv.shape)}")
+        n, width = qkv.shape
+        value_dim = int(value_dim or head_dim)
+        if n_heads <= 0 or n_kv_heads <= 0 or n_heads % n_kv_heads or n_heads > 65535:
+            raise KernelError(f"{n_heads} query heads cannot share {n_kv_heads} key/value heads evenly")
+        limit = self.core.sia_attention_generic_max_head_dim()
+        if not 0 < head_dim <= limit or not 0 < value_dim <= limit:
+            raise KernelError(f"heads of {head_dim} and values of {value_dim} are outside what the kernels take (1 to {limit})")
+        if width < n_heads * head_dim or n != ctx.n_tokens:
+            raise KernelError(f"qkv {tuple(qkv.shape)} does not hold {ctx.n_tokens} rows of {n_heads} heads of {head_dim}")
+        self._check_pages(cache.k_pages, cache.v_pages, cache.block_table, cache.page_size, n_kv_heads, head_dim, qkv.dtype, ctx,
+                          value_dim)
+        if sinks is not None:
+            self._want(sinks, "sinks", torch.float32, (n_heads,))
+        weights, max_kv = self._check_weights(cache, ctx, n_kv_heads)
+        self._same_device(qkv, cache.k_pages, cache.v_pages, cache.block_table, weights, sinks)
+        out = torch.empty((n, n_heads * value_dim), dtype=qkv.dtype, device=qkv.device)
+        if not n:
+            return out
+        table, pages = cache.block_table, cache.k_pages.shape[0]
+        stats = torch.empty((n, n_heads), dtype=torch.float32, device=qkv.device)
+        self._check(self.core.sia_attention_generic_stats(
+            _ptr(qkv), width, _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(table), table.shape[1], _ptr(ctx.seq_of_token),
+            _ptr(ctx.positions), _ptr(out), n, n_heads, n_kv_heads, head_dim, value_dim, cache.page_size, float(scale), _ptr(sinks),
+            _ptr(stats), _DT[qkv.dtype], self._stream()), "attention_generic_stats")
+        self._check(self.core.sia_weigh_plain(
+            _ptr(qkv), width, _ptr(cache.k_pages), _ptr(table), table.shape[1], _ptr(ctx.cu_q), _ptr(ctx.kv_len),
+            _ptr(ctx.state_slots), _ptr(stats), _ptr(weights), weights.shape[0], weights.shape[2], ctx.n_seqs, max_kv, n_heads,
+            n_kv_heads, head_dim, cache.page_size, pages, float(scale), _DT[qkv.dtype], self._stream()), "weigh_plain")
+        return out
+
+    def evict_cache(self, ctx, cache, budget, keep_first=0, keep_last=0):
+        """Drops what got least attention: every sequence of the step with more than ``budget`` places (``ctx.kv_len``) keeps, for
+        every key/value head by itself, its first ``keep_first`` places, its last ``keep_last`` and, of those between, the ones with the largest
+        ``cache.weights`` (ties: the lowest place; NaN counts as minus infinity), ``budget`` in all.  Keys, values and weights are
+        moved within the sequence's pages, which it must not share: with ``edge = budget - keep_last``, what is kept below the edge stays where it is, the
+        kept places from the edge on fill the holes below it, both in order, and the last ``keep_last`` move up together to the edge.  What
+        lies behind the new length stays as it was.  Returns ``(kept, lengths)``: int32 ``[n_seqs, n_kv, budget]``, the
+        place from which a place's content came (-1 behind the last), and int32 ``[n_seqs]``, the new lengths.  ``ctx`` itself is not changed: the
+        next step's places begin at the new lengths (``CacheManager.shrink`` keeps the books)."""
+        budget, keep_first, keep_last = int(budget), int(keep_first), int(keep_last)
+        if budget <= 0 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > budget:
+            raise KernelError(f"a budget of {budget} does not hold the first {keep_first} and the last {keep_last}")
+        k_pages, v_pages, table = cache.k_pages, cache.v_pages, cache.block_table
+        if k_pages is None or k_pages.dim() != 4 or v_pages is None or v_pages.dim() != 4 or k_pages.dtype not in _DT:
+            raise KernelError("the cache has no float32 or bfloat16 pages of keys and values")
+        n_kv, head_dim, value_dim = k_pages.shape[1], k_pages.shape[3], v_pages.shape[2]
+        self._check_pages(k_pages, v_pages, table, cache.page_size, n_kv, head_dim, k_pages.dtype, ctx, value_dim)
+        weights, max_kv = self._check_weights(cache, ctx, n_kv)
+        if table.shape[1] * cache.page_size < max_kv:
+            raise KernelError(f"block table {tuple(table.shape)} does not cover {max_kv} places with pages of {cache.page_size}")
+        self._same_device(k_pages, v_pages, table, weights)
+        n, device = ctx.n_seqs, weights.device
+        kept = torch.empty((n, n_kv, budget), dtype=torch.int32, device=device)
+        lengths = torch.empty((n,), dtype=torch.int32, device=device)
+        if not n:
+            return kept, lengths
+        ws = torch.empty((self.core.sia_evict_workspace(n, max_kv, n_kv, budget, keep_last),), dtype=torch.int32, device=device)
+        self._check(self.core.sia_evict(
+            _ptr(k_pages), _ptr(v_pages), _ptr(weights), _ptr(ctx.state_slots), _ptr(ctx.kv_len), _ptr(table), table.shape[1],
+            k_pages.shape[0], weights.shape[0], weights.shape[2], n, max_kv, n_kv, head_dim, value_dim, cache.page_size, budget,
+            keep_first, keep_last, _ptr(kept), _ptr(lengths), _ptr(ws), _DT[k_pages.dtype], self._stream()), "evict")
+        return kept, lengths
 
     def _attention_plan(self, lib, device, n_heads, n_kv_heads, head_dim, window, ctx, chunk=0, keep_first=0, page_size=0):
         """What the attention launches of a step need beside the tensors: the same for every layer with this

@@ -42,7 +42,8 @@ HIPCC_FLAGS = [
 LIBRARIES: Dict[str, Sequence[str]] = {
     "core": ("elementwise.hip", "rope_cache.hip", "qk_prepare.hip", "attention_generic.hip", "attention_f32.hip", "gemm_generic.hip", "gemm_f32.hip", "gemm_skinny.hip", "gemm_tiles.hip",
              "sampling.hip", "bandwidth.hip", "block.hip", "gated.hip", "recurrent.hip", "moe.hip", "dyt.hip", "conv.hip", "latent.hip",
-             "layernorm.hip", "lowrank.hip", "token_input.hip", "row_prepare.hip", "rglru.hip", "token_shift.hip"),
+             "layernorm.hip", "lowrank.hip", "token_input.hip", "row_prepare.hip", "rglru.hip", "token_shift.hip",
+             "rope_axes.hip", "attention_weighed.hip", "evict.hip"),
     # the vendor's BLAS library called directly (the products of steps of many tokens); optional: without it those
     # products go through torch
     "blas": ("library_product.hip",),

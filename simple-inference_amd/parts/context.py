@@ -62,6 +62,7 @@ class LayerCache:
     block_table: Optional[torch.Tensor] = None  # [n_seqs, max_pages] int32, -1 where no page
     page_size: int = 0
     state: Optional[torch.Tensor] = None        # [slots, *state_shape]; row = ctx.state_slots[s]
+    weights: Optional[torch.Tensor] = None      # float32 [slots, kv_heads, places]: attention weight that each cached key has got
 
 
 class ResidualStream:
