@@ -1,0 +1,413 @@
+// bfloat16 attention over the paged cache that also adds up each cached key's weight (attention_weighed.hip says what the sums are),
+// on the matrix cores.  Compiled once per head size with attention_mfma.hip, whose tiles it uses.
+//
+// Single tokens (weighed_decode_kernel): one walk over keys and values.  A weight can be made only when the row's maximum and sum are known, and
+// those only when all splits of the sequence are through: the walk leaves every scaled score (float, in units of log2) in a workspace,
+// 4 bytes a key and query head beside the 4 * head size bytes a key and key/value head that it reads, and weighed_join_kernel turns
+// them into weights while it merges the splits.  A sequence of one split is finished by its one workgroup.
+// Runs of tokens (weigh_runs_kernel): the attention kernel leaves every row's statistic, and the scores are made once more, with keys as
+// rows and queries as columns: a lane holds 4 keys of 16 columns' scores, so that the sum over the queries stays in its registers to the end.
+#include "attention_tiles.h"
+
+// ---------------------------------------------------------------------------------------------------
+// single tokens
+// ---------------------------------------------------------------------------------------------------
+// Where the sums of one (sequence, head) lie; null for a slot that is none.
+__device__ __forceinline__ float* weight_row(float* weights, const int* __restrict__ slots, int n_slots, int places, int seq, int n_kv, int hk) {
+    const int slot = slots[seq];
+    return slot < 0 || slot >= n_slots ? nullptr : weights + ((size_t)slot * n_kv + hk) * places;
+}
+
+// What a launch for single tokens is given.
+struct Weighed {
+    float* weights;           // [n_slots][key/value heads][places]
+    const int* slots;
+    float* scores;            // [sequence][query head][row_keys]
+    int n_slots, places, row_keys;
+};
+
+// Keys [j0, j1) of a sequence and head: their weights from the scores, summed over the group's query heads in order.  The last key is the
+// step's own: its sum begins at zero.
+__device__ __forceinline__ void add_weights(float* __restrict__ row, const float* __restrict__ scores, int row_keys, const float* stat, int group,
+                                            int j0, int j1, int length, int first_thread, int threads) {
+    for (int j = j0 + first_thread; j < j1; j += threads) {
+        float sum = 0.f;
+        for (int c = 0; c < group; ++c) sum += fast_exp2(scores[(size_t)c * row_keys + j] - stat[c]);
+        row[j] = (j < length - 1 ? row[j] : 0.f) + sum;
+    }
+}
+
+// Scores of a tile as they go into the workspace: lane (r, g) holds keys kb + 8 g .. + 7 of column r.
+__device__ __forceinline__ void leave_scores(float* __restrict__ mine, int kb, int g, const floatx4 (&s)[2], float scale) {
+    float4* to = reinterpret_cast<float4*>(mine + kb + 8 * g);
+    to[0] = make_float4(s[0][0] * scale, s[0][1] * scale, s[0][2] * scale, s[0][3] * scale);
+    to[1] = make_float4(s[1][0] * scale, s[1][1] * scale, s[1][2] * scale, s[1][3] * scale);
+}
+
+// Values of positions beyond `last` as zeros: pages may hold anything there, and a weight of 0 times a number without bounds is none.
+__device__ __forceinline__ void clear_values(Stage& st, int kb, int g, int last) {
+    const int n = min(max(last - (kb + 8 * g) + 1, 0), 8);      // of this lane's 8 positions
+    uint32_t keep[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) keep[i] = n >= 2 * i + 2 ? 0xffffffffu : n == 2 * i + 1 ? 0x0000ffffu : 0u;
+#pragma unroll
+    for (int db = 0; db < DBLOCKS; ++db) {
+        uint4 u = __builtin_bit_cast(uint4, st.v[db]);
+        u.x &= keep[0], u.y &= keep[1], u.z &= keep[2], u.w &= keep[3];
+        st.v[db] = __builtin_bit_cast(bf16x8, u);
+    }
+}
+
+// grid (groups of query heads, sequences, splits), four waves of a run of tiles each, as attn_decode_kernel's plain mode.
+// kv_share groups of query heads read one key/value head; with more than one, or several splits, the join makes the weights.
+__global__ __launch_bounds__(DEC_WAVES* SIA_WAVE) void weighed_decode_kernel(
+    const bf16_t* __restrict__ q, int q_row_stride, const bf16_t* __restrict__ kp, const bf16_t* __restrict__ vp,
+    const int* __restrict__ block_table, int table_width, const int* __restrict__ cu_q, const int* __restrict__ kv_len,
+    float* __restrict__ ws_acc, float* __restrict__ ws_ml, bf16_t* __restrict__ out, int n_heads, int n_groups, int ps_log2, float scale,
+    const float* __restrict__ sinks, int max_splits, int kv_share, int max_kv, const Weighed w) {
+    extern __shared__ float lds[];  // [waves][group][HD + 2]
+    const int hg = blockIdx.x, seq = blockIdx.y, split = blockIdx.z;
+    const int wave = threadIdx.x / SIA_WAVE, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int length = min(min(kv_len[seq], max_kv), min(w.places, table_width << ps_log2)), last = length - 1, group = n_heads / n_groups;
+    if (length <= 0) {      // a row that sees nothing
+        for (int i = threadIdx.x; i < group * HD && split == 0; i += DEC_WAVES * SIA_WAVE)
+            out[((size_t)cu_q[seq] * n_heads + hg * group) * HD + i] = 0;
+        return;
+    }
+    const int n_tiles = last / TILE + 1, n_splits = min(decode_splits(n_tiles), max_splits);
+    if (split >= n_splits) return;
+    scale *= LOG2E;  // exponentials are taken as powers of two
+    const int hk = hg / kv_share, n_kv = n_groups / kv_share;
+    const int* table = block_table + (size_t)seq * table_width;
+    bf16x8 qf[KSTEPS];
+    load_q(qf, r < group ? q + (size_t)seq * q_row_stride + (hg * group + r) * HD : nullptr, g);
+    const int n_runs = n_splits * DEC_WAVES, run = split * DEC_WAVES + wave;
+    const int first = (int)(((long long)run * n_tiles) / n_runs), end = (int)(((long long)(run + 1) * n_tiles) / n_runs);
+    float* const scores = w.scores + ((size_t)seq * n_heads + hg * group + min(r, group - 1)) * w.row_keys;
+
+    Softmax<1> sm;
+    sm.start();
+    floatx4 acc[1][DBLOCKS];
+#pragma unroll
+    for (int db = 0; db < DBLOCKS; ++db) acc[0][db] = floatx4{0.f, 0.f, 0.f, 0.f};
+    const Forms none{0.f, 0};
+    const Places all{0, 0};
+    const int lo[1] = {r < group ? 0 : 1 << 30}, hi[1] = {r < group ? last : -1};
+    auto compute = [&](Stage& st, int kb) {
+        floatx4 s[1][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            s[0][h] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KSTEPS; ++ks) s[0][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(st.k[h][ks], qf[ks], s[0][h], 0, 0, 0);
+        }
+        if (r < group) leave_scores(scores, kb, g, s[0], scale);
+        if (kb + TILE - 1 > last) clear_values(st, kb, g, last);
+        bf16x8 p[1];
+        softmax_update<1>(s, kb, lo, hi, scale, sm, acc, p, none);
+#pragma unroll
+        for (int db = 0; db < DBLOCKS; ++db) acc[0][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(st.v[db], p[0], acc[0][db], 0, 0, 0);
+    };
+    const int range_lo = first * TILE, range_hi = min(last, end * TILE - 1), kb_end = (end - 1) * TILE;
+    for (int w_first = range_lo; first < end && w_first <= kb_end;) {      // 64 entries of the block table at a time
+        const int first_page = w_first >> ps_log2, w_end = (first_page + SIA_WAVE) << ps_log2, w_last = min(kb_end, w_end - TILE);
+        PageWindow pages;
+        pages_load(pages, table, table_width, first_page, lane, ps_log2, all);
+        Stage a, b;
+        load_stage(a, kp, vp, pages, ps_log2, n_kv, hk, w_first, range_lo, range_hi);
+        for (int kb = w_first; kb <= w_last; kb += 2 * TILE) {      // two register stages in turn
+            load_stage(b, kp, vp, pages, ps_log2, n_kv, hk, min(kb + TILE, w_last), range_lo, range_hi);
+            compute(a, kb);
+            load_stage(a, kp, vp, pages, ps_log2, n_kv, hk, min(kb + 2 * TILE, w_last), range_lo, range_hi);
+            if (kb + TILE <= w_last) compute(b, kb + TILE);
+        }
+        w_first = w_end;
+    }
+    constexpr int ROW = HD + 2;
+    leave_state(lds + (size_t)(wave * group + min(r, group - 1)) * ROW, sm, acc, g, r < group);
+    __syncthreads();      // the states are there, and so are the workgroup's scores
+
+    __shared__ float stat[16];
+    for (int idx = threadIdx.x; idx < group * HD; idx += DEC_WAVES * SIA_WAVE) {
+        const int c = idx / HD, d = idx % HD, head = hg * group + c;
+        float o, mx, lsum;
+        merge_waves([&](int v) { return lds + (size_t)(v * group + c) * ROW; }, d, o, mx, lsum);
+        if (n_splits == 1) {
+            const float total = lsum + sink_term(sinks, head, mx);
+            out[((size_t)cu_q[seq] * n_heads + head) * HD + d] = float_to_bf16(o * (1.f / total));
+            if (d == 0) stat[c] = mx + log2f(total);
+        } else {
+            ws_acc[(((size_t)seq * n_heads + head) * max_splits + split) * HD + d] = o;
+        }
+        if (d == 0 && ws_ml) {
+            float* ml = ws_ml + (((size_t)seq * n_heads + head) * max_splits + split) * 2;
+            ml[0] = mx;
+            ml[1] = lsum;
+        }
+    }
+    if (n_splits > 1 || kv_share > 1) return;
+    __syncthreads();
+    float* row = weight_row(w.weights, w.slots, w.n_slots, w.places, seq, n_kv, hk);
+    if (row) add_weights(row, w.scores + ((size_t)seq * n_heads + hg * group) * w.row_keys, w.row_keys, stat, group, 0, length, length, threadIdx.x, DEC_WAVES * SIA_WAVE);
+}
+
+// grid (key/value heads, sequences, 1 + chunks of JOIN_KEYS keys): workgroup 0 merges the splits' results, the others make the weights
+// of their keys from the scores, with the rows' statistics made anew from the splits' (a few hundred bytes).
+constexpr int JOIN_KEYS = 512, JOIN_THREADS = 256, JOIN_MOST_HEADS = 256;
+__global__ __launch_bounds__(JOIN_THREADS) void weighed_join_kernel(
+    const float* __restrict__ ws_acc, const float* __restrict__ ws_ml, const int* __restrict__ cu_q, const int* __restrict__ kv_len,
+    bf16_t* __restrict__ out, int n_heads, int n_kv, int max_splits, int kv_share, const float* __restrict__ sinks, int max_kv, int most_keys,
+    const Weighed w) {
+    const int hk = blockIdx.x, seq = blockIdx.y, chunk = (int)blockIdx.z - 1;
+    const int length = min(min(kv_len[seq], max_kv), most_keys), group = n_heads / n_kv;
+    if (length <= 0 || chunk * JOIN_KEYS >= length) return;
+    const int n_splits = min(decode_splits((length - 1) / TILE + 1), max_splits);
+    if (n_splits == 1 && (kv_share == 1 || chunk < 0)) return;      // finished by its one workgroup
+    __shared__ float stat[JOIN_MOST_HEADS];
+    const size_t base = ((size_t)seq * n_heads + hk * group) * max_splits;
+    const float2* const ml = reinterpret_cast<const float2*>(ws_ml) + base;
+    if (chunk < 0) {
+        for (int idx = threadIdx.x; idx < group * HD; idx += JOIN_THREADS) {
+            const int c = idx / HD, d = idx % HD, head = hk * group + c;
+            float mx = -INFINITY;
+            for (int s = 0; s < n_splits; ++s) mx = fmaxf(mx, ml[(size_t)c * max_splits + s].x);
+            const float* acc_at = ws_acc + (base + (size_t)c * max_splits) * HD + d;
+            out[((size_t)cu_q[seq] * n_heads + head) * HD + d] = float_to_bf16(merge_splits(n_splits, mx, sink_term(sinks, head, mx), [&](int s, float& a, float& m, float& l) {
+                const float2 state = ml[(size_t)c * max_splits + s];
+                a = acc_at[(size_t)s * HD];
+                m = state.x;
+                l = state.y;
+            }));
+        }
+        return;
+    }
+    for (int c = threadIdx.x; c < group; c += JOIN_THREADS) {
+        float mx = -INFINITY;
+        for (int s = 0; s < n_splits; ++s) mx = fmaxf(mx, ml[(size_t)c * max_splits + s].x);
+        float total = sink_term(sinks, hk * group + c, mx);
+        for (int s = 0; s < n_splits; ++s) total = fmaf(fast_exp2(ml[(size_t)c * max_splits + s].x - mx), ml[(size_t)c * max_splits + s].y, total);
+        stat[c] = mx + log2f(total);
+    }
+    __syncthreads();
+    float* row = weight_row(w.weights, w.slots, w.n_slots, w.places, seq, n_kv, hk);
+    if (row)
+        add_weights(row, w.scores + ((size_t)seq * n_heads + hk * group) * w.row_keys, w.row_keys, stat, group, chunk * JOIN_KEYS,
+                    min(length, (chunk + 1) * JOIN_KEYS), length, threadIdx.x, JOIN_THREADS);
+}
+
+// ---------------------------------------------------------------------------------------------------
+// runs of tokens
+// ---------------------------------------------------------------------------------------------------
+// The rows of a key/value head are its (token, query head) pairs, token by token; a row sees the keys up to its token's place.  A workgroup
+// has RUN_KEYS keys, 64 a wave, held as operands, and walks the rows of a chunk 16 at a time.
+constexpr int RUN_WAVES = 4, WAVE_KEYS = 64, RUN_KEYS = RUN_WAVES * WAVE_KEYS;
+
+// Whether the chunk of rows that ends before row_end has a row that sees a key of the block at key0: the same for the kernel that writes a
+// block's sums and the one that reads them.
+__device__ __forceinline__ bool chunk_sees(int row_end, int group, int start, int key0) { return start + (row_end - 1) / group >= key0; }
+
+// grid (blocks of RUN_KEYS keys, key/value heads, chunks of chunk_rows rows of the sequences one after the other).  parts:
+// [chunk][key/value head][row_keys] the chunk's sums; or with parts == nullptr (one chunk a sequence) straight into the weights.
+__global__ __launch_bounds__(RUN_WAVES* SIA_WAVE) void weigh_runs_kernel(
+    const bf16_t* __restrict__ q, int q_row_stride, const bf16_t* __restrict__ kp, const int* __restrict__ block_table, int table_width,
+    const int* __restrict__ cu_q, const int* __restrict__ kv_len, const float* __restrict__ row_stats, int n_heads, int n_kv, int ps_log2,
+    float scale, int seq_begin, int seq_end, int chunk_rows, int max_kv, float* __restrict__ parts, const Weighed w) {
+    const int hk = blockIdx.y, group = n_heads / n_kv;
+    int seq = seq_begin, chunk = blockIdx.z;
+    for (; seq < seq_end; ++seq) {
+        const int chunks = ((cu_q[seq + 1] - cu_q[seq]) * group + chunk_rows - 1) / chunk_rows;
+        if (chunk < chunks) break;
+        chunk -= chunks;
+    }
+    if (seq >= seq_end) return;
+    const int q_begin = cu_q[seq], q_len = cu_q[seq + 1] - q_begin, length = min(min(kv_len[seq], max_kv), min(w.places, table_width << ps_log2)), start = length - q_len;
+    const int key0 = blockIdx.x * RUN_KEYS, row_end = min((chunk + 1) * chunk_rows, q_len * group);
+    if (key0 >= length || !chunk_sees(row_end, group, start, key0)) return;
+    const int wave = threadIdx.x / SIA_WAVE, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int k0 = key0 + wave * WAVE_KEYS;
+    const int* table = block_table + (size_t)seq * table_width;
+    scale *= LOG2E;
+
+    floatx4 sum[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) sum[b] = floatx4{0.f, 0.f, 0.f, 0.f};
+    if (k0 < length) {
+        bf16x8 kf[4][KSTEPS];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int key = min(k0 + b * 16 + r, length - 1);
+            const int page = max(table[key >> ps_log2], 0);
+            load_q(kf[b], kp + (((size_t)page * n_kv + hk) * (1 << ps_log2) + (key & ((1 << ps_log2) - 1))) * HD, g);
+        }
+        // from the first row that sees the wave's first key on
+        const int row_first = max(chunk * chunk_rows, max(0, k0 - start) * group);
+        // this lane's column: a row, as its token and query head; every fetch goes on by 16 rows, without a division
+        int row = row_first + r, token = row / group, head = row - token * group;
+        const int by_token = 16 / group, by_head = 16 - by_token * group, last_token = (row_end - 1) / group;
+        auto fetch = [&](bf16x8 (&qf)[KSTEPS], float& stat, int& place) {
+            const int t = min(token, last_token);       // behind the last row: some row of the last token, with weights of 0
+            const size_t at = (size_t)(q_begin + t);
+            load_q(qf, q + at * q_row_stride + (hk * group + head) * HD, g);
+            stat = row < row_end ? row_stats[at * n_heads + hk * group + head] : INFINITY;
+            place = start + t;
+            row += 16;
+            token += by_token;
+            head += by_head;
+            if (head >= group) {
+                head -= group;
+                ++token;
+            }
+        };
+        auto compute = [&](const bf16x8 (&qf)[KSTEPS], float stat, int place) {
+            floatx4 s[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                s[b] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < KSTEPS; ++ks) s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[b][ks], qf[ks], s[b], 0, 0, 0);
+            }
+            const bool whole = __all(k0 + WAVE_KEYS - 1 <= place);
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p = fast_exp2(fmaf(s[b][i], scale, -stat));
+                    sum[b][i] += whole || k0 + b * 16 + g * 4 + i <= place ? p : 0.f;
+                }
+        };
+        bf16x8 qa[KSTEPS], qb[KSTEPS];
+        float sa, sb;
+        int pa, pb;
+        if (row_first < row_end) fetch(qa, sa, pa);
+        for (int row0 = row_first; row0 < row_end; row0 += 32) {
+            fetch(qb, sb, pb);
+            compute(qa, sa, pa);
+            if (row0 + 16 >= row_end) break;
+            fetch(qa, sa, pa);
+            compute(qb, sb, pb);
+        }
+        // over the 16 columns that the lanes of a row of 16 have
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int off = 1; off < 16; off *= 2) sum[b][i] += __shfl_xor(sum[b][i], off, SIA_WAVE);
+        if (r == 0) {
+            float* to = parts ? parts + ((size_t)blockIdx.z * n_kv + hk) * w.row_keys : weight_row(w.weights, w.slots, w.n_slots, w.places, seq, n_kv, hk);
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = k0 + b * 16 + g * 4 + i;
+                    if (j < length && to) to[j] = (parts || j >= start ? 0.f : to[j]) + sum[b][i];
+                }
+        }
+    }
+}
+
+// A thread a key: the chunks that see its block, in order.
+constexpr int ADD_THREADS = 256;
+__global__ __launch_bounds__(ADD_THREADS) void weigh_runs_add_kernel(const float* __restrict__ parts, const int* __restrict__ cu_q,
+                                                                     const int* __restrict__ kv_len, int n_heads, int n_kv, int seq_begin,
+                                                                     int chunk_rows, int max_kv, const Weighed w) {
+    const int hk = blockIdx.y, seq = seq_begin + blockIdx.z, group = n_heads / n_kv, j = blockIdx.x * ADD_THREADS + threadIdx.x;
+    const int q_len = cu_q[seq + 1] - cu_q[seq], length = min(min(kv_len[seq], max_kv), w.places), start = length - q_len;
+    if (j >= length || q_len <= 0) return;
+    int first = 0;      // this sequence's first chunk
+    for (int s = seq_begin; s < seq; ++s) first += ((cu_q[s + 1] - cu_q[s]) * group + chunk_rows - 1) / chunk_rows;
+    const int rows = q_len * group, chunks = (rows + chunk_rows - 1) / chunk_rows;
+    float* row = weight_row(w.weights, w.slots, w.n_slots, w.places, seq, n_kv, hk);
+    if (!row) return;
+    float sum = 0.f;
+    for (int c = 0; c < chunks; ++c)
+        if (chunk_sees(min((c + 1) * chunk_rows, rows), group, start, j / RUN_KEYS * RUN_KEYS)) sum += parts[((size_t)(first + c) * n_kv + hk) * w.row_keys + j];
+    row[j] = (j < start ? row[j] : 0.f) + sum;
+}
+
+// ---------------------------------------------------------------------------------------------------
+// entry points
+// ---------------------------------------------------------------------------------------------------
+static int log2_of(int v) {
+    int l = 0;
+    while ((1 << l) < v && l < 30) ++l;
+    return (1 << l) == v ? l : -1;
+}
+
+// Floats from one head's scores (or one chunk's sums) to the next for sequences of up to max_kv places: whole tiles.
+static long long row_keys_of(int max_kv) { return ((long long)max_kv + TILE - 1) / TILE * TILE; }
+static int splits_of(int max_kv) { return decode_splits((max_kv + TILE - 1) / TILE); }
+
+// Groups of query heads that share a key/value head: a launch's columns are 16, and the four waves' states lie in 64 KiB.
+static int shares_of(int group) {
+    for (int s = 1; s < group; ++s)
+        if (group % s == 0 && group / s <= 16 && (size_t)DEC_WAVES * (group / s) * (HD + 2) * sizeof(float) <= 64 * 1024) return s;
+    return group;
+}
+
+SIA_EXPORT int sia_attn_weighed_max_group() { return JOIN_MOST_HEADS; }
+
+// Floats that sia_attn_weighed_decode's workspace holds.
+SIA_EXPORT long long sia_attn_weighed_decode_workspace(int n_seqs, int n_heads, int max_kv) {
+    if (n_seqs <= 0 || n_heads <= 0 || max_kv <= 0) return 0;
+    return (long long)n_seqs * n_heads * (row_keys_of(max_kv) + (long long)splits_of(max_kv) * (HD + 2));
+}
+
+// Sequences 0 .. n_seqs-1 of the step, each with one new token, which is row s of q, and none longer than max_kv; weights [n_slots][n_kv]
+// [places], a sequence's row at slots[s].
+SIA_EXPORT int sia_attn_weighed_decode(const void* q, int q_row_stride, const void* k_pages, const void* v_pages, const int* block_table,
+                                       int table_width, const int* cu_q, const int* kv_len, void* out, float* ws, int n_seqs, int n_heads, int n_kv,
+                                       int page_size, float scale, const float* sinks, int max_kv, float* weights, const int* slots, int n_slots,
+                                       int places, hipStream_t stream) {
+    if (n_seqs <= 0) return 0;
+    const int ps_log2 = log2_of(page_size);
+    if (ps_log2 < 3 || n_kv <= 0 || n_heads % n_kv || n_heads / n_kv > JOIN_MOST_HEADS || n_heads > 65535 || n_seqs > 65535 || q_row_stride % 8 || table_width <= 0 ||
+        max_kv <= 0 || places < max_kv || n_slots <= 0 || !ws || !weights || !(scale > 0.f))
+        return SIA_BAD_ARGUMENT;
+    const int share = shares_of(n_heads / n_kv), n_groups = n_kv * share, max_splits = splits_of(max_kv);
+    const Weighed w{weights, slots, ws, n_slots, places, (int)row_keys_of(max_kv)};
+    float* acc = ws + (long long)n_seqs * n_heads * w.row_keys;
+    float* ml = acc + (long long)n_seqs * n_heads * max_splits * HD;
+    const size_t lds_bytes = (size_t)DEC_WAVES * (n_heads / n_groups) * (HD + 2) * sizeof(float);
+    hipLaunchKernelGGL(weighed_decode_kernel, dim3(n_groups, n_seqs, max_splits), dim3(DEC_WAVES * SIA_WAVE), lds_bytes, stream, (const bf16_t*)q,
+                       q_row_stride, (const bf16_t*)k_pages, (const bf16_t*)v_pages, block_table, table_width, cu_q, kv_len, acc, ml, (bf16_t*)out,
+                       n_heads, n_groups, ps_log2, scale, sinks, max_splits, share, max_kv, w);
+    if (max_splits > 1 || share > 1)
+        hipLaunchKernelGGL(weighed_join_kernel, dim3(n_kv, n_seqs, 1 + (max_kv + JOIN_KEYS - 1) / JOIN_KEYS), dim3(JOIN_THREADS), 0, stream, acc, ml,
+                           cu_q, kv_len, (bf16_t*)out, n_heads, n_kv, max_splits, share, sinks, max_kv, (int)min((long long)places, (long long)table_width << ps_log2), w);
+    return SIA_LAUNCH_CHECK();
+}
+
+// Rows of a key/value head that one workgroup walks: enough workgroups to fill the chip several times over, none with so few rows that its keys'
+// loads count.  blocks: of RUN_KEYS keys, of the longest sequence.
+SIA_EXPORT int sia_weigh_runs_chunk(int total_rows, int n_kv, int max_kv) {
+    const long long blocks = ((long long)max_kv + RUN_KEYS - 1) / RUN_KEYS;
+    const long long rows = (long long)total_rows * n_kv * blocks / 2048;
+    return (int)(rows < 256 ? 256 : (rows + 63) / 64 * 64);
+}
+
+// Floats of the workspace for n_chunks chunks in all (0: every sequence has one).
+SIA_EXPORT long long sia_weigh_runs_workspace(int n_chunks, int n_runs, int n_kv, int max_kv) {
+    return n_chunks <= n_runs ? 0 : (long long)n_chunks * n_kv * row_keys_of(max_kv);
+}
+
+// Sequences seq_begin .. seq_end-1, none longer than max_kv; n_chunks: the sum over them of ceil(tokens * n_heads / n_kv / chunk_rows).
+SIA_EXPORT int sia_weigh_runs(const void* q, int q_row_stride, const void* k_pages, const int* block_table, int table_width, const int* cu_q,
+                              const int* kv_len, const float* row_stats, float* ws, int seq_begin, int seq_end, int n_heads, int n_kv,
+                              int page_size, float scale, int chunk_rows, int n_chunks, int max_kv, float* weights, const int* slots, int n_slots,
+                              int places, hipStream_t stream) {
+    if (seq_end <= seq_begin || n_chunks <= 0) return 0;
+    const int ps_log2 = log2_of(page_size), n_runs = seq_end - seq_begin;
+    if (ps_log2 < 3 || n_kv <= 0 || n_heads % n_kv || n_kv > 65535 || n_chunks > 65535 || n_runs > 65535 || q_row_stride % 8 || table_width <= 0 || max_kv <= 0 || places < max_kv ||
+        n_slots <= 0 || chunk_rows <= 0 || !row_stats || !weights || (n_chunks > n_runs && !ws))
+        return SIA_BAD_ARGUMENT;
+    const Weighed w{weights, slots, nullptr, n_slots, places, (int)row_keys_of(max_kv)};
+    float* parts = n_chunks > n_runs ? ws : nullptr;
+    hipLaunchKernelGGL(weigh_runs_kernel, dim3((max_kv + RUN_KEYS - 1) / RUN_KEYS, n_kv, n_chunks), dim3(RUN_WAVES * SIA_WAVE), 0, stream,
+                       (const bf16_t*)q, q_row_stride, (const bf16_t*)k_pages, block_table, table_width, cu_q, kv_len, row_stats, n_heads, n_kv,
+                       ps_log2, scale, seq_begin, seq_end, chunk_rows, max_kv, parts, w);
+    if (parts)
+        hipLaunchKernelGGL(weigh_runs_add_kernel, dim3((max_kv + ADD_THREADS - 1) / ADD_THREADS, n_kv, n_runs), dim3(ADD_THREADS), 0, stream, parts,
+                           cu_q, kv_len, n_heads, n_kv, seq_begin, chunk_rows, max_kv, w);
+    return SIA_LAUNCH_CHECK();
+}

@@ -213,6 +213,9 @@ _ATTN_SIGNATURES = {
     "sia_attn_prefill_forms": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr,
                                _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float,
                                _c_int, _c_int, _c_ptr, _c_float, _c_int, _c_ptr],
+    "sia_attn_prefill_stats": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr,
+                               _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float,
+                               _c_ptr, _c_ptr, _c_ptr],
     "sia_attn_decode_walk": [_c_int, _c_int, _c_int],
     "sia_attn_mfma_forms": [],
     "sia_attn_decode_max_splits": [_c_int, _c_int],
@@ -225,11 +228,24 @@ _ATTN_SIGNATURES = {
     "sia_attn_mfma_head_dim": [],
 }
 
+# of the libraries without the forms
+_WEIGHED_SIGNATURES = {
+    "sia_attn_weighed_max_group": [],
+    "sia_attn_weighed_decode_workspace": [_c_int, _c_int, _c_int],
+    "sia_attn_weighed_decode": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int,
+                                _c_int, _c_float, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
+    "sia_weigh_runs_chunk": [_c_int, _c_int, _c_int],
+    "sia_weigh_runs_workspace": [_c_int, _c_int, _c_int, _c_int],
+    "sia_weigh_runs": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int,
+                       _c_float, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
+}
+
 
 def attention_library_spec(head_dim: int, forms: bool = False):
     """(name, sources, defines) of the matrix-core attention library for one head size; ``forms``: the build that also
     takes a soft cap on the scores and kept first positions."""
-    return (f"attn_mfma_d{head_dim}{'_forms' if forms else ''}", ("attention_mfma.hip",),
+    sources = ("attention_mfma.hip",) + (() if forms else ("attention_weighed_mfma.hip",))
+    return (f"attn_mfma_d{head_dim}{'_forms' if forms else ''}", sources,
             (f"SIA_HEAD_DIM={head_dim}",) + (("SIA_SCORE_FORMS=1",) if forms else ()))
 
 
@@ -408,6 +424,9 @@ class HipKernels:
             lib = build.load_library(name, sources, defines)
             _bind(lib, _ATTN_SIGNATURES)
             lib.sia_attn_decode_workspace.restype = ctypes.c_longlong
+            if not forms:
+                _bind(lib, _WEIGHED_SIGNATURES)
+                lib.sia_attn_weighed_decode_workspace.restype = lib.sia_weigh_runs_workspace.restype = ctypes.c_longlong
             if lib.sia_attn_mfma_head_dim() != head_dim or bool(lib.sia_attn_mfma_forms()) != forms:
                 raise KernelError(f"library {name} was built for another head size or other forms")
             self._attn_libs[(head_dim, forms)] = lib
@@ -2068,7 +2087,12 @@ class HipKernels:
         out = torch.empty((n, n_heads * value_dim), dtype=qkv.dtype, device=qkv.device)
         if not n:
             return out
-        table, pages = cache.block_table, cache.k_pages.shape[0]
+        table, pages, page = cache.block_table, cache.k_pages.shape[0], cache.page_size
+        if (self.use_mfma_attention and qkv.dtype == torch.bfloat16 and head_dim % 16 == 0 and head_dim <= 256 and value_dim == head_dim
+                and page >= 8 and page & (page - 1) == 0 and width % 8 == 0 and scale > 0 and n_heads // n_kv_heads <= 256
+                and _in_pieces(qkv, cache.k_pages, cache.v_pages)):
+            self._weighed_mfma(qkv, out, n_heads, n_kv_heads, head_dim, float(scale), ctx, cache, sinks, weights, max_kv)
+            return out
         stats = torch.empty((n, n_heads), dtype=torch.float32, device=qkv.device)
         self._check(self.core.sia_attention_generic_stats(
             _ptr(qkv), width, _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(table), table.shape[1], _ptr(ctx.seq_of_token),
@@ -2079,6 +2103,35 @@ class HipKernels:
             _ptr(ctx.state_slots), _ptr(stats), _ptr(weights), weights.shape[0], weights.shape[2], ctx.n_seqs, max_kv, n_heads,
             n_kv_heads, head_dim, cache.page_size, pages, float(scale), _DT[qkv.dtype], self._stream()), "weigh_plain")
         return out
+
+    def _weighed_mfma(self, qkv, out, n_heads, n_kv, head_dim, scale, ctx, cache, sinks, weights, max_kv):
+        """Single tokens by one walk over keys and values, runs by the attention kernel and the scores once more."""
+        lib, n_dec, device = self._attn_lib(head_dim), ctx.n_decode_seqs, qkv.device
+        table, page, stream = cache.block_table, cache.page_size, self._stream()
+        slots, places = weights.shape[0], weights.shape[2]
+        if n_dec:
+            ws = torch.empty((lib.sia_attn_weighed_decode_workspace(n_dec, n_heads, max_kv),), dtype=torch.float32, device=device)
+            self._check(lib.sia_attn_weighed_decode(
+                _ptr(qkv), qkv.shape[1], _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(table), table.shape[1], _ptr(ctx.cu_q),
+                _ptr(ctx.kv_len), _ptr(out), _ptr(ws), n_dec, n_heads, n_kv, page, scale, _ptr(sinks), max_kv, _ptr(weights),
+                _ptr(ctx.state_slots), slots, places, stream), "attn_weighed_decode")
+        if n_dec >= ctx.n_seqs:
+            return
+        stats = torch.empty((ctx.n_tokens, n_heads), dtype=torch.float32, device=device)
+        tiles, q_bound, kv_bound = self._run_tiles(lib, ctx)
+        self._check(lib.sia_attn_prefill_stats(
+            _ptr(qkv), qkv.shape[1], _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(table), table.shape[1], _ptr(ctx.cu_q),
+            _ptr(ctx.kv_len), _ptr(out), n_dec, ctx.n_seqs, *tiles, q_bound, kv_bound, n_heads, n_kv, page, scale, _ptr(sinks),
+            _ptr(stats), stream), "attn_prefill_stats")
+        group = n_heads // n_kv
+        chunk = lib.sia_weigh_runs_chunk(sum(ctx.q_lens[n_dec:]) * group, n_kv, kv_bound)
+        chunks, runs = sum(-(-q * group // chunk) for q in ctx.q_lens[n_dec:]), ctx.n_seqs - n_dec
+        floats = lib.sia_weigh_runs_workspace(chunks, runs, n_kv, kv_bound)
+        ws = torch.empty((floats,), dtype=torch.float32, device=device) if floats else None
+        self._check(lib.sia_weigh_runs(
+            _ptr(qkv), qkv.shape[1], _ptr(cache.k_pages), _ptr(table), table.shape[1], _ptr(ctx.cu_q), _ptr(ctx.kv_len), _ptr(stats),
+            _ptr(ws), n_dec, ctx.n_seqs, n_heads, n_kv, page, scale, chunk, chunks, kv_bound, _ptr(weights), _ptr(ctx.state_slots),
+            slots, places, stream), "weigh_runs")
 
     def evict_cache(self, ctx, cache, budget, keep_first=0, keep_last=0):
         """Drops what got least attention: every sequence of the step with more than ``budget`` places (``ctx.kv_len``) keeps, for
@@ -2113,6 +2166,14 @@ class HipKernels:
             keep_first, keep_last, _ptr(kept), _ptr(lengths), _ptr(ws), _DT[k_pages.dtype], self._stream()), "evict")
         return kept, lengths
 
+    @staticmethod
+    def _run_tiles(lib, ctx):
+        """Row tiles of the step's runs at each of the prefill kernel's workgroup sizes, and the most tokens and keys of one."""
+        runs = ctx.q_lens[ctx.n_decode_seqs:]
+        tiles = tuple(sum(-(-q // rows) for q in runs) if rows else 0
+                      for rows in (lib.sia_attn_prefill_rows(), lib.sia_attn_prefill_rows_split(), lib.sia_attn_prefill_rows_long()))
+        return tiles, int(max(runs)), int(getattr(ctx, "max_run_kv_len", 0) or ctx.max_kv_len)
+
     def _attention_plan(self, lib, device, n_heads, n_kv_heads, head_dim, window, ctx, chunk=0, keep_first=0, page_size=0):
         """What the attention launches of a step need beside the tensors: the same for every layer with this
         geometry, so it is worked out once per step and kept with the step's context (workspaces included: a step's
@@ -2143,10 +2204,8 @@ class HipKernels:
         if n_dec < ctx.n_seqs:
             # row tiles at each of the kernel's workgroup sizes, and what bounds a sequence's tokens and keys in this
             # step: a portion over a long past takes another workgroup shape than a prompt from its start
-            tiles = tuple(sum(-(-q // rows) for q in ctx.q_lens[n_dec:]) if rows else 0
-                          for rows in (lib.sia_attn_prefill_rows(), lib.sia_attn_prefill_rows_split(),
-                                       lib.sia_attn_prefill_rows_long()))
-            tiles += (int(max(ctx.q_lens[n_dec:])), int(getattr(ctx, "max_run_kv_len", 0) or ctx.max_kv_len))
+            tiles, *bounds = self._run_tiles(lib, ctx)
+            tiles += tuple(bounds)
         plan = (n_dec, max_splits, ws_acc, ws_ml, tiles, share)
         if plans is None:
             try:
