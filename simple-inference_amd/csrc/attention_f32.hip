@@ -17,30 +17,12 @@
 #include <algorithm>
 #include <cmath>
 
-#include "common.h"
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+#include "f32_lanes.h"
 
 #define CHUNK SIA_WAVE      // keys at a time
 #define WAVES 4
 #define ROWS 16             // (token, head) pairs of a workgroup
 #define P_ROW (CHUNK + 4)
-
-// Lane (r, g) = 16 g + r holds elements 4 g .. 4 g + 3 of its row; afterwards element e of it is element 4 e + g of the row: the order in which
-// four steps of the matrix instruction take them.  And the other way round.
-__device__ __forceinline__ void across_groups(f32x4& x) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const u32x2 v = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[e]), __float_as_uint(x[e + 2]), false, false);
-        x[e] = __uint_as_float(v[0]), x[e + 2] = __uint_as_float(v[1]);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; e += 2) {
-        const u32x2 v = __builtin_amdgcn_permlane16_swap(__float_as_uint(x[e]), __float_as_uint(x[e + 1]), false, false);
-        x[e] = __uint_as_float(v[0]), x[e + 1] = __uint_as_float(v[1]);
-    }
-}
 
 // x of this lane and x of the lane OFF away (16 or 32), one way round or the other
 template <int OFF>
@@ -71,7 +53,7 @@ __global__ __launch_bounds__(WAVES * SIA_WAVE) void attention_f32_kernel(
     const int* __restrict__ block_table, int table_width, const int* __restrict__ seq_of_token,
     const int* __restrict__ positions, float* __restrict__ out, int n_tokens, int n_single, int n_heads, int n_kv,
     int head_dim, int value_dim, int page_size, float scale, int window, int chunk, const float* __restrict__ sinks,
-    float cap, int keep_first, int tile_rows) {
+    float cap, int keep_first, int tile_rows, float* __restrict__ row_stats) {
     constexpr int PIECES = DP / 16, BLOCKS = DP < 64 ? 1 : DP / 64;      // a lane's fours of a row of keys; blocks of 16 dimensions of a wave's values
     __shared__ float most[WAVES][ROWS];
     __shared__ __attribute__((aligned(16))) float weight[ROWS * P_ROW];      // [row][position: 16 (j % 4) + j / 4]
@@ -269,6 +251,7 @@ __global__ __launch_bounds__(WAVES * SIA_WAVE) void attention_f32_kernel(
     }
     if (r >= n_rows) return;
     if (sinks) l += expf(sinks[head] - m);
+    if (row_stats && wave == 0 && g == 0) row_stats[(size_t)token * n_heads + head] = row_stat(m, l);
     const float inv = 1.f / l;
     float* o = out + ((size_t)token * n_heads + head) * value_dim;
 #pragma unroll
@@ -292,17 +275,19 @@ template <int DP>
 static int launch(const float* q, int q_row_stride, const float* k_pages, const float* v_pages, const int* block_table,
                   int table_width, const int* seq_of_token, const int* positions, float* out, int n_tokens, int n_single,
                   int n_heads, int n_kv, int head_dim, int value_dim, int page_size, float scale,
-                  int window, int chunk, const float* sinks, float cap, int keep_first, int tile_rows, hipStream_t stream) {
+                  int window, int chunk, const float* sinks, float cap, int keep_first, int tile_rows, float* row_stats, hipStream_t stream) {
     const long long tiles = tiles_of(n_tokens, n_single, n_heads / n_kv, tile_rows);
     if (tiles * n_kv > 0x7fffffff) return SIA_BAD_ARGUMENT;
     hipLaunchKernelGGL(attention_f32_kernel<DP>, dim3((unsigned)(tiles * n_kv)), dim3(WAVES * SIA_WAVE), 0, stream, q, q_row_stride, k_pages,
                        v_pages, block_table, table_width, seq_of_token, positions, out, n_tokens, n_single, n_heads, n_kv, head_dim,
-                       value_dim, page_size, scale, window, chunk, sinks, cap, keep_first, tile_rows);
+                       value_dim, page_size, scale, window, chunk, sinks, cap, keep_first, tile_rows, row_stats);
     return SIA_LAUNCH_CHECK();
 }
 
 extern "C" int sia_attention_generic(const void*, int, const void*, const void*, const int*, int, const int*, const int*, void*,
                                      int, int, int, int, int, int, float, int, int, const float*, float, int, int, hipStream_t);
+extern "C" int sia_attention_generic_stats(const void*, int, const void*, const void*, const int*, int, const int*, const int*, void*,
+                                           int, int, int, int, int, int, float, const float*, float*, int, hipStream_t);
 
 // The arguments of the plain kernel, and n_single: that many tokens, the first ones, are their sequences' only ones; n_seqs;
 // max_kv: no sequence holds more keys.
@@ -312,11 +297,11 @@ extern "C" int sia_attention_generic(const void*, int, const void*, const void*,
 // do those whose workgroups here would have one row of 16 each (a query head for every key/value head) in more than a round over the chip, with keys that
 // fill no chunk:  256 tokens over 17 and 33 keys, plain and here, 16 heads of 64 on 16 22.9 / 38.9 and 28.5 / 39.8 (64 keys: 58 / 40), 40 of 96 on 40 70 / 161
 // and 152 / 185;  64 tokens, 16 of 64 7.7 / 11.5 and 11.3 / 11.7.
-SIA_EXPORT int sia_attention_f32(const float* q, int q_row_stride, const float* k_pages, const float* v_pages,
-                                 const int* block_table, int table_width, const int* seq_of_token, const int* positions,
-                                 float* out, int n_tokens, int n_single, int n_seqs, int max_kv, int n_heads, int n_kv,
-                                 int head_dim, int value_dim, int page_size, float scale, int window, int chunk, const float* sinks, float cap,
-                                 int keep_first, hipStream_t stream) {
+static int attend_f32(const float* q, int q_row_stride, const float* k_pages, const float* v_pages,
+                      const int* block_table, int table_width, const int* seq_of_token, const int* positions,
+                      float* out, int n_tokens, int n_single, int n_seqs, int max_kv, int n_heads, int n_kv,
+                      int head_dim, int value_dim, int page_size, float scale, int window, int chunk, const float* sinks, float cap,
+                      int keep_first, float* row_stats, hipStream_t stream) {
     if (n_tokens <= 0) return 0;
     const bool takes = head_dim > 0 && head_dim <= 128 && head_dim % 4 == 0 && value_dim > 0 && value_dim <= 128 &&
                        q_row_stride % 4 == 0 && page_size >= 4 && (page_size & (page_size - 1)) == 0 && n_kv > 0 &&
@@ -324,6 +309,9 @@ SIA_EXPORT int sia_attention_f32(const float* q, int q_row_stride, const float* 
                        !(max_kv <= 16 && (long long)n_tokens * n_heads <= 4096) &&
                        ((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0;
     auto plain = [&]() {
+        if (row_stats)      // (which go without window, blocks, cap and kept positions)
+            return sia_attention_generic_stats(q, q_row_stride, k_pages, v_pages, block_table, table_width, seq_of_token, positions, out,
+                                               n_tokens, n_heads, n_kv, head_dim, value_dim, page_size, scale, sinks, row_stats, SIA_F32, stream);
         return sia_attention_generic(q, q_row_stride, k_pages, v_pages, block_table, table_width, seq_of_token, positions, out,
                                      n_tokens, n_heads, n_kv, head_dim, value_dim, page_size, scale, window, chunk, sinks,
                                      cap, keep_first, SIA_F32, stream);
@@ -353,5 +341,25 @@ SIA_EXPORT int sia_attention_f32(const float* q, int q_row_stride, const float* 
     const int widest = max(head_dim, value_dim);
     return (widest <= 32 ? launch<32> : widest <= 64 ? launch<64> : launch<128>)(
         q, q_row_stride, k_pages, v_pages, block_table, table_width, seq_of_token, positions, out, n_tokens, n_single, n_heads, n_kv,
-        head_dim, value_dim, page_size, scale, window, chunk, sinks, cap, keep_first, tile_rows, stream);
+        head_dim, value_dim, page_size, scale, window, chunk, sinks, cap, keep_first, tile_rows, row_stats, stream);
+}
+
+SIA_EXPORT int sia_attention_f32(const float* q, int q_row_stride, const float* k_pages, const float* v_pages,
+                                 const int* block_table, int table_width, const int* seq_of_token, const int* positions,
+                                 float* out, int n_tokens, int n_single, int n_seqs, int max_kv, int n_heads, int n_kv,
+                                 int head_dim, int value_dim, int page_size, float scale, int window, int chunk, const float* sinks, float cap,
+                                 int keep_first, hipStream_t stream) {
+    return attend_f32(q, q_row_stride, k_pages, v_pages, block_table, table_width, seq_of_token, positions, out, n_tokens, n_single, n_seqs,
+                      max_kv, n_heads, n_kv, head_dim, value_dim, page_size, scale, window, chunk, sinks, cap, keep_first, nullptr, stream);
+}
+
+// The same without window, blocks, cap and kept positions, and the rows' statistics beside the result (float [n_tokens][n_heads]).
+SIA_EXPORT int sia_attention_f32_stats(const float* q, int q_row_stride, const float* k_pages, const float* v_pages,
+                                       const int* block_table, int table_width, const int* seq_of_token, const int* positions,
+                                       float* out, int n_tokens, int n_single, int n_seqs, int max_kv, int n_heads, int n_kv,
+                                       int head_dim, int value_dim, int page_size, float scale, const float* sinks, float* row_stats,
+                                       hipStream_t stream) {
+    if (!row_stats) return SIA_BAD_ARGUMENT;
+    return attend_f32(q, q_row_stride, k_pages, v_pages, block_table, table_width, seq_of_token, positions, out, n_tokens, n_single, n_seqs,
+                      max_kv, n_heads, n_kv, head_dim, value_dim, page_size, scale, 0, 0, sinks, 0.f, 0, row_stats, stream);
 }

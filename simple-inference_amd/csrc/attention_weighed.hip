@@ -7,34 +7,31 @@
 // the values is needed, only the scores again.  A place that the step itself has written begins at zero, whatever lay there.
 // All sums are float, each made by one thread in a fixed order.
 //
+// Float heads of up to 128 go by the float matrix cores (weigh_f32_kernel), with keys as rows and queries as columns, single tokens and
+// runs alike; bfloat16 heads of 16 to 256 by attention_weighed_mfma.hip.
 // The plain kernel: a wave for 64 consecutive places of one (sequence, key/value head), a lane a key; the queries come one after
 // the other through LDS.  It takes every head size, page size and type.
-#include "common.h"
+#include "f32_lanes.h"
+#include "weighed.h"
 
 #define WEIGH_MAX_HEAD_DIM 640
-
-// Where the sums of one (sequence, head) lie; null for a slot that is none.
-__device__ __forceinline__ float* weight_row(float* weights, const int* __restrict__ slots, int n_slots, int places, int seq, int n_kv, int hk) {
-    const int slot = slots[seq];
-    return slot < 0 || slot >= n_slots ? nullptr : weights + ((size_t)slot * n_kv + hk) * places;
-}
 
 template <typename T>
 __global__ __launch_bounds__(SIA_WAVE) void weigh_plain_kernel(
     const T* __restrict__ q, int q_row_stride, const T* __restrict__ k_pages, const int* __restrict__ block_table, int table_width,
-    const int* __restrict__ cu_q, const int* __restrict__ kv_len, const int* __restrict__ slots, const float* __restrict__ row_stats,
-    float* __restrict__ weights, int n_slots, int places, int n_heads, int n_kv, int head_dim, int page_size, int n_pages, float scale) {
+    const int* __restrict__ cu_q, const int* __restrict__ kv_len, const float* __restrict__ row_stats, int n_heads, int n_kv, int head_dim,
+    int page_size, int n_pages, float scale, const Weighed w) {
     __shared__ float q_s[WEIGH_MAX_HEAD_DIM];
     const int lane = threadIdx.x, hk = blockIdx.y, seq = blockIdx.z, group = n_heads / n_kv;
-    const int first = cu_q[seq], n = cu_q[seq + 1] - first, length = min(kv_len[seq], places), start = length - n;
+    const int first = cu_q[seq], n = cu_q[seq + 1] - first, length = min(kv_len[seq], w.places), start = length - n;
     const int j0 = blockIdx.x * SIA_WAVE, j = j0 + lane;
-    float* row = weight_row(weights, slots, n_slots, places, seq, n_kv, hk);
+    float* row = weight_row(w, seq, n_kv, hk);
     if (j0 >= length || !row) return;
     int page = j < length && j / page_size < table_width ? block_table[(size_t)seq * table_width + j / page_size] : -1;
     if (page >= n_pages) page = -1;
     const T* key = k_pages + (((size_t)max(page, 0) * n_kv + hk) * page_size + j % page_size) * head_dim;
-    float sum = 0.f;
-    for (int t = max(0, j0 - start); t < n; ++t)
+    float total = 0.f, sum = 0.f;      // of tokens, and of 64 of them: a long run's small weights are not added one by one to a large sum
+    for (int t = max(0, j0 - start); t < n; ++t) {
         for (int h = hk * group; h < (hk + 1) * group; ++h) {
             const T* q_row = q + (size_t)(first + t) * q_row_stride + h * head_dim;
             for (int d = lane; d < head_dim; d += SIA_WAVE) q_s[d] = to_float(q_row[d]);
@@ -46,7 +43,12 @@ __global__ __launch_bounds__(SIA_WAVE) void weigh_plain_kernel(
             sum += page >= 0 && j <= start + t ? p : 0.f;
             __syncthreads();
         }
-    if (j < length) row[j] = (j < start ? row[j] : 0.f) + sum;
+        if (t % 64 == 63 || t == n - 1) {
+            total += sum;
+            sum = 0.f;
+        }
+    }
+    if (j < length) row[j] = (j < start ? row[j] : 0.f) + total;
 }
 
 // q: rows of the step's tokens, n_heads * head_dim columns first; cu_q, kv_len, slots: per sequence; row_stats [tokens][n_heads];
@@ -59,14 +61,148 @@ SIA_EXPORT int sia_weigh_plain(const void* q, int q_row_stride, const void* k_pa
     if (head_dim <= 0 || head_dim > WEIGH_MAX_HEAD_DIM || n_kv <= 0 || n_heads % n_kv || page_size <= 0 || n_kv > 65535 || n_seqs > 65535 ||
         places <= 0 || table_width <= 0 || n_pages <= 0)
         return SIA_BAD_ARGUMENT;
+    const Weighed w{weights, slots, nullptr, n_slots, places, 0};
     const dim3 grid((max_kv + SIA_WAVE - 1) / SIA_WAVE, n_kv, n_seqs);
 #define LAUNCH(T)                                                                                                                   \
     hipLaunchKernelGGL(weigh_plain_kernel<T>, grid, dim3(SIA_WAVE), 0, stream, (const T*)q, q_row_stride, (const T*)k_pages,        \
-                       block_table, table_width, cu_q, kv_len, slots, row_stats, weights, n_slots, places, n_heads, n_kv, head_dim, \
-                       page_size, n_pages, scale)
+                       block_table, table_width, cu_q, kv_len, row_stats, n_heads, n_kv, head_dim, page_size, n_pages, scale, w)
     if (dtype == SIA_F32) LAUNCH(float);
     else if (dtype == SIA_BF16) LAUNCH(bf16_t);
     else return SIA_BAD_ARGUMENT;
 #undef LAUNCH
+    return SIA_LAUNCH_CHECK();
+}
+
+// ---------------------------------------------------------------------------------------------------
+// float heads of up to 128 on the float matrix cores (v_mfma_f32_16x16x4_f32)
+// ---------------------------------------------------------------------------------------------------
+// A dot product's elements come in the attention kernels' order, so that a score has the bits that went into its row's statistic: what is
+// left of a weight's error is that of two exponentials and a sum.  (In the order in which a lane loads them, without the exchange between
+// lanes, errors of 8e-7 of the sums where 2e-7 are now.)
+constexpr int F32_WAVES = 4, F32_BLOCKS = 2, F32_WAVE_KEYS = 16 * F32_BLOCKS, F32_KEYS = F32_WAVES * F32_WAVE_KEYS;
+
+// DP: 32, 64 or 128, the head sizes' upper bound.  grid and parts as weigh_runs_kernel's.
+template <int DP>
+__global__ __launch_bounds__(F32_WAVES* SIA_WAVE) void weigh_f32_kernel(
+    const float* __restrict__ q, int q_row_stride, const float* __restrict__ k_pages, const int* __restrict__ block_table, int table_width,
+    const int* __restrict__ cu_q, const int* __restrict__ kv_len, const float* __restrict__ row_stats, int n_heads, int n_kv, int head_dim,
+    int page_size, int n_pages, float scale, int n_seqs, int chunk_rows, int most_keys, float* __restrict__ parts, const Weighed w) {
+    constexpr int PIECES = DP / 16;
+    const int hk = blockIdx.y, group = n_heads / n_kv, key0 = blockIdx.x * F32_KEYS;
+    Run run;
+    if (!find_run(run, blockIdx.z, cu_q, kv_len, 0, n_seqs, group, chunk_rows, most_keys)) return;
+    if (key0 >= run.length || !chunk_sees(run.row_end, group, run.start, key0)) return;
+    const int wave = threadIdx.x / SIA_WAVE, lane = threadIdx.x % SIA_WAVE, r = lane & 15, g = lane >> 4;
+    const int k0 = key0 + wave * F32_WAVE_KEYS;
+    if (k0 >= run.length) return;
+    const int* table = block_table + (size_t)run.seq * table_width;
+    auto load_row = [&](f32x4 (&x)[PIECES], const float* row) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int d = 16 * i + 4 * g;
+            x[i] = *(const f32x4*)(row + (d < head_dim ? d : 0));
+            if (d >= head_dim) x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            across_groups(x[i]);
+        }
+    };
+    f32x4 sum[F32_BLOCKS], kf[F32_BLOCKS][PIECES];
+    bool paged[F32_BLOCKS];
+#pragma unroll
+    for (int b = 0; b < F32_BLOCKS; ++b) {
+        sum[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int key = min(k0 + b * 16 + r, run.length - 1), page = table[key / page_size];
+        paged[b] = page >= 0 && page < n_pages;
+        load_row(kf[b], k_pages + (((size_t)(paged[b] ? page : 0) * n_kv + hk) * page_size + key % page_size) * head_dim);
+    }
+    // the places beyond which this lane's four keys of a block are seen by none: where there is no page, nobody's
+    int seen_from[F32_BLOCKS][4];
+#pragma unroll
+    for (int b = 0; b < F32_BLOCKS; ++b) {
+        const unsigned long long pages = __ballot(paged[b]);      // lanes 0 .. 15: the block's keys
+#pragma unroll
+        for (int i = 0; i < 4; ++i) seen_from[b][i] = pages >> (4 * g + i) & 1 ? k0 + b * 16 + 4 * g + i : 0x7fffffff;
+    }
+    const int row_first = max(run.chunk * chunk_rows, max(0, k0 - run.start) * group), by_token = 16 / group, by_head = 16 - by_token * group;
+    const int last_token = (run.row_end - 1) / group;
+    Column col;
+    col.begin(row_first + r, group);
+    auto fetch = [&](f32x4 (&qf)[PIECES], float& stat, int& place) {
+        const int t = min(col.token, last_token);      // behind the last row: some row of the last token, with weights of 0
+        const size_t at = (size_t)(run.q_begin + t);
+        load_row(qf, q + at * q_row_stride + (hk * group + col.head) * head_dim);
+        stat = col.row < run.row_end ? row_stats[at * n_heads + hk * group + col.head] : INFINITY;
+        place = run.start + t;
+        col.next(by_token, by_head, group);
+    };
+    f32x4 qa[PIECES], qb[PIECES];
+    float sa, sb;
+    int pa, pb;
+    auto compute = [&](const f32x4 (&qf)[PIECES], float stat, int place) {
+        f32x4 s[F32_BLOCKS];
+#pragma unroll
+        for (int b = 0; b < F32_BLOCKS; ++b) s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int b = 0; b < F32_BLOCKS; ++b) s[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[b][i][e], qf[i][e], s[b], 0, 0, 0);
+#pragma unroll
+        for (int b = 0; b < F32_BLOCKS; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = exp2f(fmaf(s[b][i] * scale, 1.4426950408889634f, -stat));
+                sum[b][i] += seen_from[b][i] <= place ? p : 0.f;
+            }
+    };
+    if (row_first < run.row_end) fetch(qa, sa, pa);
+    for (int row0 = row_first; row0 < run.row_end; row0 += 32) {
+        fetch(qb, sb, pb);
+        compute(qa, sa, pa);
+        if (row0 + 16 >= run.row_end) break;
+        fetch(qa, sa, pa);
+        compute(qb, sb, pb);
+    }
+    leave_sums(sum, k0, run, parts ? parts + ((size_t)blockIdx.z * n_kv + hk) * w.row_keys : nullptr, w, n_kv, hk);
+}
+
+// Whether weigh_f32_kernel takes such heads (and rows of q and keys in sixteens of bytes).
+SIA_EXPORT int sia_weigh_f32_takes(int head_dim) { return head_dim > 0 && head_dim <= 128 && head_dim % 4 == 0; }
+
+// Rows of a key/value head that one workgroup walks: enough workgroups to fill the chip several times over.
+SIA_EXPORT int sia_weigh_f32_chunk(int total_rows, int n_kv, int max_kv) {
+    const long long blocks = ((long long)max_kv + F32_KEYS - 1) / F32_KEYS, rows = (long long)total_rows * n_kv * blocks / 2048;
+    return (int)(rows < 64 ? 64 : (rows + 15) / 16 * 16);
+}
+
+// Floats of the workspace for n_chunks chunks in all (0: no sequence has more than one).
+SIA_EXPORT long long sia_weigh_f32_workspace(int n_chunks, int n_seqs, int n_kv, int max_kv) {
+    return n_chunks <= n_seqs ? 0 : (long long)n_chunks * n_kv * max_kv;
+}
+
+// As sia_weigh_plain; n_chunks: the sum over the sequences of ceil(tokens * n_heads / n_kv / chunk_rows).
+SIA_EXPORT int sia_weigh_f32(const float* q, int q_row_stride, const float* k_pages, const int* block_table, int table_width, const int* cu_q,
+                             const int* kv_len, const int* slots, const float* row_stats, float* weights, int n_slots, int places, int n_seqs,
+                             int max_kv, int n_heads, int n_kv, int head_dim, int page_size, int n_pages, float scale, int chunk_rows, int n_chunks,
+                             float* ws, hipStream_t stream) {
+    if (n_seqs <= 0 || max_kv <= 0 || n_chunks <= 0) return 0;
+    if (!sia_weigh_f32_takes(head_dim) || q_row_stride % 4 || ((uintptr_t)q | (uintptr_t)k_pages) % 16 || n_kv <= 0 || n_heads % n_kv || page_size <= 0 ||
+        n_kv > 65535 || n_seqs > 65535 || n_chunks > 65535 || places < max_kv || table_width <= 0 || n_pages <= 0 || n_slots <= 0 || chunk_rows <= 0 ||
+        (n_chunks > n_seqs && !ws))
+        return SIA_BAD_ARGUMENT;
+    const Weighed w{weights, slots, nullptr, n_slots, places, max_kv};
+    const int most_keys = (int)min((long long)max_kv, (long long)table_width * page_size);
+    float* parts = n_chunks > n_seqs ? ws : nullptr;
+#define LAUNCH(DP)                                                                                                                          \
+    hipLaunchKernelGGL(weigh_f32_kernel<DP>, dim3((max_kv + F32_KEYS - 1) / F32_KEYS, n_kv, n_chunks), dim3(F32_WAVES * SIA_WAVE), 0, stream, q, \
+                       q_row_stride, k_pages, block_table, table_width, cu_q, kv_len, row_stats, n_heads, n_kv, head_dim, page_size, n_pages,  \
+                       scale, n_seqs, chunk_rows, most_keys, parts, w)
+    if (head_dim <= 32) LAUNCH(32);
+    else if (head_dim <= 64) LAUNCH(64);
+    else LAUNCH(128);
+#undef LAUNCH
+    if (parts)
+        hipLaunchKernelGGL(weigh_runs_add_kernel<F32_KEYS>, dim3((max_kv + ADD_THREADS - 1) / ADD_THREADS, n_kv, n_seqs), dim3(ADD_THREADS), 0, stream,
+                           parts, cu_q, kv_len, n_heads, n_kv, 0, chunk_rows, most_keys, w);
     return SIA_LAUNCH_CHECK();
 }

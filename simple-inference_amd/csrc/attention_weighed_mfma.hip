@@ -8,24 +8,11 @@
 // Runs of tokens (weigh_runs_kernel): the attention kernel leaves every row's statistic, and the scores are made once more, with keys as
 // rows and queries as columns: a lane holds 4 keys of 16 columns' scores, so that the sum over the queries stays in its registers to the end.
 #include "attention_tiles.h"
+#include "weighed.h"
 
 // ---------------------------------------------------------------------------------------------------
 // single tokens
 // ---------------------------------------------------------------------------------------------------
-// Where the sums of one (sequence, head) lie; null for a slot that is none.
-__device__ __forceinline__ float* weight_row(float* weights, const int* __restrict__ slots, int n_slots, int places, int seq, int n_kv, int hk) {
-    const int slot = slots[seq];
-    return slot < 0 || slot >= n_slots ? nullptr : weights + ((size_t)slot * n_kv + hk) * places;
-}
-
-// What a launch for single tokens is given.
-struct Weighed {
-    float* weights;           // [n_slots][key/value heads][places]
-    const int* slots;
-    float* scores;            // [sequence][query head][row_keys]
-    int n_slots, places, row_keys;
-};
-
 // Keys [j0, j1) of a sequence and head: their weights from the scores, summed over the group's query heads in order.  The last key is the
 // step's own: its sum begins at zero.
 __device__ __forceinline__ void add_weights(float* __restrict__ row, const float* __restrict__ scores, int row_keys, const float* stat, int group,
@@ -64,11 +51,11 @@ __global__ __launch_bounds__(DEC_WAVES* SIA_WAVE) void weighed_decode_kernel(
     const bf16_t* __restrict__ q, int q_row_stride, const bf16_t* __restrict__ kp, const bf16_t* __restrict__ vp,
     const int* __restrict__ block_table, int table_width, const int* __restrict__ cu_q, const int* __restrict__ kv_len,
     float* __restrict__ ws_acc, float* __restrict__ ws_ml, bf16_t* __restrict__ out, int n_heads, int n_groups, int ps_log2, float scale,
-    const float* __restrict__ sinks, int max_splits, int kv_share, int max_kv, const Weighed w) {
+    const float* __restrict__ sinks, int max_splits, int kv_share, int most_keys, const Weighed w) {
     extern __shared__ float lds[];  // [waves][group][HD + 2]
     const int hg = blockIdx.x, seq = blockIdx.y, split = blockIdx.z;
     const int wave = threadIdx.x / SIA_WAVE, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const int length = min(min(kv_len[seq], max_kv), min(w.places, table_width << ps_log2)), last = length - 1, group = n_heads / n_groups;
+    const int length = min(kv_len[seq], most_keys), last = length - 1, group = n_heads / n_groups;
     if (length <= 0) {      // a row that sees nothing
         for (int i = threadIdx.x; i < group * HD && split == 0; i += DEC_WAVES * SIA_WAVE)
             out[((size_t)cu_q[seq] * n_heads + hg * group) * HD + i] = 0;
@@ -147,7 +134,7 @@ __global__ __launch_bounds__(DEC_WAVES* SIA_WAVE) void weighed_decode_kernel(
     }
     if (n_splits > 1 || kv_share > 1) return;
     __syncthreads();
-    float* row = weight_row(w.weights, w.slots, w.n_slots, w.places, seq, n_kv, hk);
+    float* row = weight_row(w, seq, n_kv, hk);
     if (row) add_weights(row, w.scores + ((size_t)seq * n_heads + hg * group) * w.row_keys, w.row_keys, stat, group, 0, length, length, threadIdx.x, DEC_WAVES * SIA_WAVE);
 }
 
@@ -156,10 +143,10 @@ __global__ __launch_bounds__(DEC_WAVES* SIA_WAVE) void weighed_decode_kernel(
 constexpr int JOIN_KEYS = 512, JOIN_THREADS = 256, JOIN_MOST_HEADS = 256;
 __global__ __launch_bounds__(JOIN_THREADS) void weighed_join_kernel(
     const float* __restrict__ ws_acc, const float* __restrict__ ws_ml, const int* __restrict__ cu_q, const int* __restrict__ kv_len,
-    bf16_t* __restrict__ out, int n_heads, int n_kv, int max_splits, int kv_share, const float* __restrict__ sinks, int max_kv, int most_keys,
+    bf16_t* __restrict__ out, int n_heads, int n_kv, int max_splits, int kv_share, const float* __restrict__ sinks, int most_keys,
     const Weighed w) {
     const int hk = blockIdx.x, seq = blockIdx.y, chunk = (int)blockIdx.z - 1;
-    const int length = min(min(kv_len[seq], max_kv), most_keys), group = n_heads / n_kv;
+    const int length = min(kv_len[seq], most_keys), group = n_heads / n_kv;
     if (length <= 0 || chunk * JOIN_KEYS >= length) return;
     const int n_splits = min(decode_splits((length - 1) / TILE + 1), max_splits);
     if (n_splits == 1 && (kv_share == 1 || chunk < 0)) return;      // finished by its one workgroup
@@ -189,7 +176,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void weighed_join_kernel(
         stat[c] = mx + log2f(total);
     }
     __syncthreads();
-    float* row = weight_row(w.weights, w.slots, w.n_slots, w.places, seq, n_kv, hk);
+    float* row = weight_row(w, seq, n_kv, hk);
     if (row)
         add_weights(row, w.scores + ((size_t)seq * n_heads + hk * group) * w.row_keys, w.row_keys, stat, group, chunk * JOIN_KEYS,
                     min(length, (chunk + 1) * JOIN_KEYS), length, threadIdx.x, JOIN_THREADS);
@@ -198,131 +185,75 @@ __global__ __launch_bounds__(JOIN_THREADS) void weighed_join_kernel(
 // ---------------------------------------------------------------------------------------------------
 // runs of tokens
 // ---------------------------------------------------------------------------------------------------
-// The rows of a key/value head are its (token, query head) pairs, token by token; a row sees the keys up to its token's place.  A workgroup
-// has RUN_KEYS keys, 64 a wave, held as operands, and walks the rows of a chunk 16 at a time.
-constexpr int RUN_WAVES = 4, WAVE_KEYS = 64, RUN_KEYS = RUN_WAVES * WAVE_KEYS;
+constexpr int RUN_WAVES = 4, WAVE_BLOCKS = 4, WAVE_KEYS = 16 * WAVE_BLOCKS, RUN_KEYS = RUN_WAVES * WAVE_KEYS;
 
-// Whether the chunk of rows that ends before row_end has a row that sees a key of the block at key0: the same for the kernel that writes a
-// block's sums and the one that reads them.
-__device__ __forceinline__ bool chunk_sees(int row_end, int group, int start, int key0) { return start + (row_end - 1) / group >= key0; }
-
-// grid (blocks of RUN_KEYS keys, key/value heads, chunks of chunk_rows rows of the sequences one after the other).  parts:
-// [chunk][key/value head][row_keys] the chunk's sums; or with parts == nullptr (one chunk a sequence) straight into the weights.
+// grid (blocks of RUN_KEYS keys, key/value heads, chunks of chunk_rows rows of the sequences one after the other); a wave holds its 64 keys as
+// operands and walks the rows 16 at a time.  parts: [chunk][key/value head][row_keys], or null where every sequence has one chunk.
 __global__ __launch_bounds__(RUN_WAVES* SIA_WAVE) void weigh_runs_kernel(
     const bf16_t* __restrict__ q, int q_row_stride, const bf16_t* __restrict__ kp, const int* __restrict__ block_table, int table_width,
     const int* __restrict__ cu_q, const int* __restrict__ kv_len, const float* __restrict__ row_stats, int n_heads, int n_kv, int ps_log2,
-    float scale, int seq_begin, int seq_end, int chunk_rows, int max_kv, float* __restrict__ parts, const Weighed w) {
-    const int hk = blockIdx.y, group = n_heads / n_kv;
-    int seq = seq_begin, chunk = blockIdx.z;
-    for (; seq < seq_end; ++seq) {
-        const int chunks = ((cu_q[seq + 1] - cu_q[seq]) * group + chunk_rows - 1) / chunk_rows;
-        if (chunk < chunks) break;
-        chunk -= chunks;
-    }
-    if (seq >= seq_end) return;
-    const int q_begin = cu_q[seq], q_len = cu_q[seq + 1] - q_begin, length = min(min(kv_len[seq], max_kv), min(w.places, table_width << ps_log2)), start = length - q_len;
-    const int key0 = blockIdx.x * RUN_KEYS, row_end = min((chunk + 1) * chunk_rows, q_len * group);
-    if (key0 >= length || !chunk_sees(row_end, group, start, key0)) return;
+    float scale, int seq_begin, int seq_end, int chunk_rows, int most_keys, float* __restrict__ parts, const Weighed w) {
+    const int hk = blockIdx.y, group = n_heads / n_kv, key0 = blockIdx.x * RUN_KEYS;
+    Run run;
+    if (!find_run(run, blockIdx.z, cu_q, kv_len, seq_begin, seq_end, group, chunk_rows, most_keys)) return;
+    if (key0 >= run.length || !chunk_sees(run.row_end, group, run.start, key0)) return;
     const int wave = threadIdx.x / SIA_WAVE, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int k0 = key0 + wave * WAVE_KEYS;
-    const int* table = block_table + (size_t)seq * table_width;
+    if (k0 >= run.length) return;
+    const int* table = block_table + (size_t)run.seq * table_width;
     scale *= LOG2E;
 
-    floatx4 sum[4];
+    floatx4 sum[WAVE_BLOCKS];
+    bf16x8 kf[WAVE_BLOCKS][KSTEPS];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) sum[b] = floatx4{0.f, 0.f, 0.f, 0.f};
-    if (k0 < length) {
-        bf16x8 kf[4][KSTEPS];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int key = min(k0 + b * 16 + r, length - 1);
-            const int page = max(table[key >> ps_log2], 0);
-            load_q(kf[b], kp + (((size_t)page * n_kv + hk) * (1 << ps_log2) + (key & ((1 << ps_log2) - 1))) * HD, g);
-        }
-        // from the first row that sees the wave's first key on
-        const int row_first = max(chunk * chunk_rows, max(0, k0 - start) * group);
-        // this lane's column: a row, as its token and query head; every fetch goes on by 16 rows, without a division
-        int row = row_first + r, token = row / group, head = row - token * group;
-        const int by_token = 16 / group, by_head = 16 - by_token * group, last_token = (row_end - 1) / group;
-        auto fetch = [&](bf16x8 (&qf)[KSTEPS], float& stat, int& place) {
-            const int t = min(token, last_token);       // behind the last row: some row of the last token, with weights of 0
-            const size_t at = (size_t)(q_begin + t);
-            load_q(qf, q + at * q_row_stride + (hk * group + head) * HD, g);
-            stat = row < row_end ? row_stats[at * n_heads + hk * group + head] : INFINITY;
-            place = start + t;
-            row += 16;
-            token += by_token;
-            head += by_head;
-            if (head >= group) {
-                head -= group;
-                ++token;
-            }
-        };
-        auto compute = [&](const bf16x8 (&qf)[KSTEPS], float stat, int place) {
-            floatx4 s[4];
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                s[b] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int ks = 0; ks < KSTEPS; ++ks) s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[b][ks], qf[ks], s[b], 0, 0, 0);
-            }
-            const bool whole = __all(k0 + WAVE_KEYS - 1 <= place);
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float p = fast_exp2(fmaf(s[b][i], scale, -stat));
-                    sum[b][i] += whole || k0 + b * 16 + g * 4 + i <= place ? p : 0.f;
-                }
-        };
-        bf16x8 qa[KSTEPS], qb[KSTEPS];
-        float sa, sb;
-        int pa, pb;
-        if (row_first < row_end) fetch(qa, sa, pa);
-        for (int row0 = row_first; row0 < row_end; row0 += 32) {
-            fetch(qb, sb, pb);
-            compute(qa, sa, pa);
-            if (row0 + 16 >= row_end) break;
-            fetch(qa, sa, pa);
-            compute(qb, sb, pb);
-        }
-        // over the 16 columns that the lanes of a row of 16 have
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int off = 1; off < 16; off *= 2) sum[b][i] += __shfl_xor(sum[b][i], off, SIA_WAVE);
-        if (r == 0) {
-            float* to = parts ? parts + ((size_t)blockIdx.z * n_kv + hk) * w.row_keys : weight_row(w.weights, w.slots, w.n_slots, w.places, seq, n_kv, hk);
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int j = k0 + b * 16 + g * 4 + i;
-                    if (j < length && to) to[j] = (parts || j >= start ? 0.f : to[j]) + sum[b][i];
-                }
-        }
+    for (int b = 0; b < WAVE_BLOCKS; ++b) {
+        sum[b] = floatx4{0.f, 0.f, 0.f, 0.f};
+        const int key = min(k0 + b * 16 + r, run.length - 1);
+        const int page = max(table[key >> ps_log2], 0);
+        load_q(kf[b], kp + (((size_t)page * n_kv + hk) * (1 << ps_log2) + (key & ((1 << ps_log2) - 1))) * HD, g);
     }
-}
-
-// A thread a key: the chunks that see its block, in order.
-constexpr int ADD_THREADS = 256;
-__global__ __launch_bounds__(ADD_THREADS) void weigh_runs_add_kernel(const float* __restrict__ parts, const int* __restrict__ cu_q,
-                                                                     const int* __restrict__ kv_len, int n_heads, int n_kv, int seq_begin,
-                                                                     int chunk_rows, int max_kv, const Weighed w) {
-    const int hk = blockIdx.y, seq = seq_begin + blockIdx.z, group = n_heads / n_kv, j = blockIdx.x * ADD_THREADS + threadIdx.x;
-    const int q_len = cu_q[seq + 1] - cu_q[seq], length = min(min(kv_len[seq], max_kv), w.places), start = length - q_len;
-    if (j >= length || q_len <= 0) return;
-    int first = 0;      // this sequence's first chunk
-    for (int s = seq_begin; s < seq; ++s) first += ((cu_q[s + 1] - cu_q[s]) * group + chunk_rows - 1) / chunk_rows;
-    const int rows = q_len * group, chunks = (rows + chunk_rows - 1) / chunk_rows;
-    float* row = weight_row(w.weights, w.slots, w.n_slots, w.places, seq, n_kv, hk);
-    if (!row) return;
-    float sum = 0.f;
-    for (int c = 0; c < chunks; ++c)
-        if (chunk_sees(min((c + 1) * chunk_rows, rows), group, start, j / RUN_KEYS * RUN_KEYS)) sum += parts[((size_t)(first + c) * n_kv + hk) * w.row_keys + j];
-    row[j] = (j < start ? row[j] : 0.f) + sum;
+    // from the first row that sees the wave's first key on
+    const int row_first = max(run.chunk * chunk_rows, max(0, k0 - run.start) * group), by_token = 16 / group, by_head = 16 - by_token * group;
+    const int last_token = (run.row_end - 1) / group;
+    Column col;
+    col.begin(row_first + r, group);
+    auto fetch = [&](bf16x8 (&qf)[KSTEPS], float& stat, int& place) {
+        const int t = min(col.token, last_token);       // behind the last row: some row of the last token, with weights of 0
+        const size_t at = (size_t)(run.q_begin + t);
+        load_q(qf, q + at * q_row_stride + (hk * group + col.head) * HD, g);
+        stat = col.row < run.row_end ? row_stats[at * n_heads + hk * group + col.head] : INFINITY;
+        place = run.start + t;
+        col.next(by_token, by_head, group);
+    };
+    auto compute = [&](const bf16x8 (&qf)[KSTEPS], float stat, int place) {
+        floatx4 s[WAVE_BLOCKS];
+#pragma unroll
+        for (int b = 0; b < WAVE_BLOCKS; ++b) {
+            s[b] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KSTEPS; ++ks) s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[b][ks], qf[ks], s[b], 0, 0, 0);
+        }
+        const bool whole = __all(k0 + WAVE_KEYS - 1 <= place);
+#pragma unroll
+        for (int b = 0; b < WAVE_BLOCKS; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = fast_exp2(fmaf(s[b][i], scale, -stat));
+                sum[b][i] += whole || k0 + b * 16 + g * 4 + i <= place ? p : 0.f;
+            }
+    };
+    bf16x8 qa[KSTEPS], qb[KSTEPS];
+    float sa, sb;
+    int pa, pb;
+    if (row_first < run.row_end) fetch(qa, sa, pa);
+    for (int row0 = row_first; row0 < run.row_end; row0 += 32) {      // the next 16 rows on their way while these are computed
+        fetch(qb, sb, pb);
+        compute(qa, sa, pa);
+        if (row0 + 16 >= run.row_end) break;
+        fetch(qa, sa, pa);
+        compute(qb, sb, pb);
+    }
+    leave_sums(sum, k0, run, parts ? parts + ((size_t)blockIdx.z * n_kv + hk) * w.row_keys : nullptr, w, n_kv, hk);
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -366,15 +297,16 @@ SIA_EXPORT int sia_attn_weighed_decode(const void* q, int q_row_stride, const vo
         return SIA_BAD_ARGUMENT;
     const int share = shares_of(n_heads / n_kv), n_groups = n_kv * share, max_splits = splits_of(max_kv);
     const Weighed w{weights, slots, ws, n_slots, places, (int)row_keys_of(max_kv)};
+    const int most_keys = (int)min((long long)max_kv, (long long)table_width << ps_log2);      // what there is room for, whatever kv_len says
     float* acc = ws + (long long)n_seqs * n_heads * w.row_keys;
     float* ml = acc + (long long)n_seqs * n_heads * max_splits * HD;
     const size_t lds_bytes = (size_t)DEC_WAVES * (n_heads / n_groups) * (HD + 2) * sizeof(float);
     hipLaunchKernelGGL(weighed_decode_kernel, dim3(n_groups, n_seqs, max_splits), dim3(DEC_WAVES * SIA_WAVE), lds_bytes, stream, (const bf16_t*)q,
                        q_row_stride, (const bf16_t*)k_pages, (const bf16_t*)v_pages, block_table, table_width, cu_q, kv_len, acc, ml, (bf16_t*)out,
-                       n_heads, n_groups, ps_log2, scale, sinks, max_splits, share, max_kv, w);
+                       n_heads, n_groups, ps_log2, scale, sinks, max_splits, share, most_keys, w);
     if (max_splits > 1 || share > 1)
         hipLaunchKernelGGL(weighed_join_kernel, dim3(n_kv, n_seqs, 1 + (max_kv + JOIN_KEYS - 1) / JOIN_KEYS), dim3(JOIN_THREADS), 0, stream, acc, ml,
-                           cu_q, kv_len, (bf16_t*)out, n_heads, n_kv, max_splits, share, sinks, max_kv, (int)min((long long)places, (long long)table_width << ps_log2), w);
+                           cu_q, kv_len, (bf16_t*)out, n_heads, n_kv, max_splits, share, sinks, most_keys, w);
     return SIA_LAUNCH_CHECK();
 }
 
@@ -402,12 +334,13 @@ SIA_EXPORT int sia_weigh_runs(const void* q, int q_row_stride, const void* k_pag
         n_slots <= 0 || chunk_rows <= 0 || !row_stats || !weights || (n_chunks > n_runs && !ws))
         return SIA_BAD_ARGUMENT;
     const Weighed w{weights, slots, nullptr, n_slots, places, (int)row_keys_of(max_kv)};
+    const int most_keys = (int)min((long long)max_kv, (long long)table_width << ps_log2);
     float* parts = n_chunks > n_runs ? ws : nullptr;
     hipLaunchKernelGGL(weigh_runs_kernel, dim3((max_kv + RUN_KEYS - 1) / RUN_KEYS, n_kv, n_chunks), dim3(RUN_WAVES * SIA_WAVE), 0, stream,
                        (const bf16_t*)q, q_row_stride, (const bf16_t*)k_pages, block_table, table_width, cu_q, kv_len, row_stats, n_heads, n_kv,
-                       ps_log2, scale, seq_begin, seq_end, chunk_rows, max_kv, parts, w);
+                       ps_log2, scale, seq_begin, seq_end, chunk_rows, most_keys, parts, w);
     if (parts)
-        hipLaunchKernelGGL(weigh_runs_add_kernel, dim3((max_kv + ADD_THREADS - 1) / ADD_THREADS, n_kv, n_runs), dim3(ADD_THREADS), 0, stream, parts,
-                           cu_q, kv_len, n_heads, n_kv, seq_begin, chunk_rows, max_kv, w);
+        hipLaunchKernelGGL(weigh_runs_add_kernel<RUN_KEYS>, dim3((max_kv + ADD_THREADS - 1) / ADD_THREADS, n_kv, n_runs), dim3(ADD_THREADS), 0, stream,
+                           parts, cu_q, kv_len, n_heads, n_kv, seq_begin, chunk_rows, most_keys, w);
     return SIA_LAUNCH_CHECK();
 }

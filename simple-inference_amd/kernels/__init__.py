@@ -113,6 +113,13 @@ _SIGNATURES = {
                                     _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_ptr, _c_int, _c_ptr],
     "sia_weigh_plain": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
                         _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_ptr],
+    "sia_attention_f32_stats": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
+                                _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_ptr, _c_ptr],
+    "sia_weigh_f32_takes": [_c_int],
+    "sia_weigh_f32_chunk": [_c_int, _c_int, _c_int],
+    "sia_weigh_f32_workspace": [_c_int, _c_int, _c_int, _c_int],
+    "sia_weigh_f32": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
+                      _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
     "sia_rope_axes_max": [],
     "sia_rope_axes_kv_write": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int,
                                _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr],
@@ -350,7 +357,7 @@ class HipKernels:
         self.core.sia_delta_rule_workspace.restype = ctypes.c_longlong
         self.core.sia_linear_unit_workspace.restype = ctypes.c_longlong
         self.core.sia_bonus_recurrence_workspace.restype = ctypes.c_longlong
-        self.core.sia_evict_workspace.restype = ctypes.c_longlong
+        self.core.sia_evict_workspace.restype = self.core.sia_weigh_f32_workspace.restype = ctypes.c_longlong
         self.tiled_experts = True        # many slots in bfloat16: experts' products on the matrix cores, slots sorted by expert
         self._attn_libs = {}
         # the short way to the current stream's handle, where this torch has it (a few microseconds less a launch)
@@ -446,13 +453,13 @@ class HipKernels:
             raise KernelError(f"{what}: HIP error {code}")
 
     def _want(self, t: torch.Tensor, what: str, dtype=None, shape=None):
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise KernelError(f"{what} must be on the GPU, is on {t.device}")
         if not t.is_contiguous():
             raise KernelError(f"{what} must be contiguous")
         if dtype is not None and t.dtype != dtype:
             raise KernelError(f"{what} must be {dtype}, is {t.dtype}")
-        if shape is not None and tuple(t.shape) != tuple(shape):
+        if shape is not None and t.shape != tuple(shape):
             raise KernelError(f"{what} must have shape {tuple(shape)}, has {tuple(t.shape)}")
 
     # -- measurement -----------------------------------------------------------
@@ -2094,14 +2101,32 @@ class HipKernels:
             self._weighed_mfma(qkv, out, n_heads, n_kv_heads, head_dim, float(scale), ctx, cache, sinks, weights, max_kv)
             return out
         stats = torch.empty((n, n_heads), dtype=torch.float32, device=qkv.device)
-        self._check(self.core.sia_attention_generic_stats(
-            _ptr(qkv), width, _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(table), table.shape[1], _ptr(ctx.seq_of_token),
-            _ptr(ctx.positions), _ptr(out), n, n_heads, n_kv_heads, head_dim, value_dim, cache.page_size, float(scale), _ptr(sinks),
-            _ptr(stats), _DT[qkv.dtype], self._stream()), "attention_generic_stats")
+        stream, places = self._stream(), (weights.shape[0], weights.shape[2])
+        if qkv.dtype == torch.float32:
+            self._check(self.core.sia_attention_f32_stats(
+                _ptr(qkv), width, _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(table), table.shape[1], _ptr(ctx.seq_of_token),
+                _ptr(ctx.positions), _ptr(out), n, ctx.n_decode_seqs, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim, value_dim, page,
+                float(scale), _ptr(sinks), _ptr(stats), stream), "attention_f32_stats")
+            if self.core.sia_weigh_f32_takes(head_dim) and width % 4 == 0 and _in_pieces(qkv, cache.k_pages):
+                group = n_heads // n_kv_heads
+                chunk = self.core.sia_weigh_f32_chunk(n * group, n_kv_heads, max_kv)
+                chunks = sum(-(-q * group // chunk) for q in ctx.q_lens)
+                floats = self.core.sia_weigh_f32_workspace(chunks, ctx.n_seqs, n_kv_heads, max_kv)
+                ws = torch.empty((floats,), dtype=torch.float32, device=qkv.device) if floats else None
+                self._check(self.core.sia_weigh_f32(
+                    _ptr(qkv), width, _ptr(cache.k_pages), _ptr(table), table.shape[1], _ptr(ctx.cu_q), _ptr(ctx.kv_len),
+                    _ptr(ctx.state_slots), _ptr(stats), _ptr(weights), *places, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim, page,
+                    pages, float(scale), chunk, chunks, _ptr(ws), stream), "weigh_f32")
+                return out
+        else:
+            self._check(self.core.sia_attention_generic_stats(
+                _ptr(qkv), width, _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(table), table.shape[1], _ptr(ctx.seq_of_token),
+                _ptr(ctx.positions), _ptr(out), n, n_heads, n_kv_heads, head_dim, value_dim, page, float(scale), _ptr(sinks), _ptr(stats),
+                _DT[qkv.dtype], stream), "attention_generic_stats")
         self._check(self.core.sia_weigh_plain(
             _ptr(qkv), width, _ptr(cache.k_pages), _ptr(table), table.shape[1], _ptr(ctx.cu_q), _ptr(ctx.kv_len),
-            _ptr(ctx.state_slots), _ptr(stats), _ptr(weights), weights.shape[0], weights.shape[2], ctx.n_seqs, max_kv, n_heads,
-            n_kv_heads, head_dim, cache.page_size, pages, float(scale), _DT[qkv.dtype], self._stream()), "weigh_plain")
+            _ptr(ctx.state_slots), _ptr(stats), _ptr(weights), *places, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim, page, pages,
+            float(scale), _DT[qkv.dtype], stream), "weigh_plain")
         return out
 
     def _weighed_mfma(self, qkv, out, n_heads, n_kv, head_dim, scale, ctx, cache, sinks, weights, max_kv):
