@@ -86,14 +86,13 @@ template <int DP>
 __global__ __launch_bounds__(F32_WAVES* SIA_WAVE) void weigh_f32_kernel(
     const float* __restrict__ q, int q_row_stride, const float* __restrict__ k_pages, const int* __restrict__ block_table, int table_width,
     const int* __restrict__ cu_q, const int* __restrict__ kv_len, const float* __restrict__ row_stats, int n_heads, int n_kv, int head_dim,
-    int page_size, int n_pages, float scale, int n_seqs, int chunk_rows, int most_keys, float* __restrict__ parts, const Weighed w) {
+    int page_size, int n_pages, float scale, int chunk_rows, int most_keys, float* __restrict__ parts, const Weighed w) {
     constexpr int PIECES = DP / 16;
-    const int hk = blockIdx.y, group = n_heads / n_kv, key0 = blockIdx.x * F32_KEYS;
-    Run run;
-    if (!find_run(run, blockIdx.z, cu_q, kv_len, 0, n_seqs, group, chunk_rows, most_keys)) return;
-    if (key0 >= run.length || !chunk_sees(run.row_end, group, run.start, key0)) return;
+    const int hk = blockIdx.x, group = n_heads / n_kv;
+    Work run;
+    if (!find_work<F32_KEYS>(run, blockIdx.y, blockIdx.z, cu_q, kv_len, group, chunk_rows, most_keys)) return;
     const int wave = threadIdx.x / SIA_WAVE, lane = threadIdx.x % SIA_WAVE, r = lane & 15, g = lane >> 4;
-    const int k0 = key0 + wave * F32_WAVE_KEYS;
+    const int k0 = run.key0 + wave * F32_WAVE_KEYS;
     if (k0 >= run.length) return;
     const int* table = block_table + (size_t)run.seq * table_width;
     auto load_row = [&](f32x4 (&x)[PIECES], const float* row) {
@@ -122,17 +121,19 @@ __global__ __launch_bounds__(F32_WAVES* SIA_WAVE) void weigh_f32_kernel(
 #pragma unroll
         for (int i = 0; i < 4; ++i) seen_from[b][i] = pages >> (4 * g + i) & 1 ? k0 + b * 16 + 4 * g + i : 0x7fffffff;
     }
-    const int row_first = max(run.chunk * chunk_rows, max(0, k0 - run.start) * group), by_token = 16 / group, by_head = 16 - by_token * group;
-    const int last_token = (run.row_end - 1) / group;
+    // from the chunk's first row that sees the wave's first key on
+    const int row_first = max(run.row_begin, max(0, k0 - run.start) * group), by_token = 16 / group, by_head = 16 - by_token * group;
+    const int last_token = max(run.row_end - 1, 0) / group;
     Column col;
     col.begin(row_first + r, group);
     auto fetch = [&](f32x4 (&qf)[PIECES], float& stat, int& place) {
         const int t = min(col.token, last_token);      // behind the last row: some row of the last token, with weights of 0
         const size_t at = (size_t)(run.q_begin + t);
         load_row(qf, q + at * q_row_stride + (hk * group + col.head) * head_dim);
-        stat = col.row < run.row_end ? row_stats[at * n_heads + hk * group + col.head] : INFINITY;
+        const float own = row_stats[at * n_heads + hk * group + col.head];
+        stat = col.row < run.row_end ? own : INFINITY;
         place = run.start + t;
-        col.next(by_token, by_head, group);
+        col.next<16>(by_token, by_head, group);
     };
     f32x4 qa[PIECES], qb[PIECES];
     float sa, sb;
@@ -163,46 +164,48 @@ __global__ __launch_bounds__(F32_WAVES* SIA_WAVE) void weigh_f32_kernel(
         fetch(qa, sa, pa);
         compute(qb, sb, pb);
     }
-    leave_sums(sum, k0, run, parts ? parts + ((size_t)blockIdx.z * n_kv + hk) * w.row_keys : nullptr, w, n_kv, hk);
+    leave_sums(sum, k0, run, parts ? parts + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * n_kv + hk) * F32_KEYS : nullptr, w, n_kv, hk);
 }
 
 // Whether weigh_f32_kernel takes such heads (and rows of q and keys in sixteens of bytes).
 SIA_EXPORT int sia_weigh_f32_takes(int head_dim) { return head_dim > 0 && head_dim <= 128 && head_dim % 4 == 0; }
 
-// Rows of a key/value head that one workgroup walks: enough workgroups to fill the chip several times over.
-SIA_EXPORT int sia_weigh_f32_chunk(int total_rows, int n_kv, int max_kv) {
-    const long long blocks = ((long long)max_kv + F32_KEYS - 1) / F32_KEYS, rows = (long long)total_rows * n_kv * blocks / 2048;
-    return (int)(rows < 64 ? 64 : (rows + 15) / 16 * 16);
+// How the sequences of a launch are cut: three workgroups are on a compute unit at a time.
+static Cut cut_f32(int total_tokens, int q_bound, int n_seqs, int max_kv, int n_heads, int n_kv) {
+    return cut_runs(total_tokens, q_bound, n_seqs, max_kv, n_heads / n_kv, n_kv, F32_KEYS, 64, 768);
 }
 
-// Floats of the workspace for n_chunks chunks in all (0: no sequence has more than one).
-SIA_EXPORT long long sia_weigh_f32_workspace(int n_chunks, int n_seqs, int n_kv, int max_kv) {
-    return n_chunks <= n_seqs ? 0 : (long long)n_chunks * n_kv * max_kv;
+// Floats of sia_weigh_f32's workspace (0: none).
+SIA_EXPORT long long sia_weigh_f32_workspace(int total_tokens, int q_bound, int n_seqs, int max_kv, int n_heads, int n_kv) {
+    if (total_tokens <= 0 || q_bound <= 0 || n_seqs <= 0 || max_kv <= 0 || n_kv <= 0 || n_heads % n_kv) return 0;
+    return cut_f32(total_tokens, q_bound, n_seqs, max_kv, n_heads, n_kv).floats;
 }
 
-// As sia_weigh_plain; n_chunks: the sum over the sequences of ceil(tokens * n_heads / n_kv / chunk_rows).
+// As sia_weigh_plain, single tokens and runs alike; total_tokens in all, no sequence with more than q_bound tokens.
 SIA_EXPORT int sia_weigh_f32(const float* q, int q_row_stride, const float* k_pages, const int* block_table, int table_width, const int* cu_q,
                              const int* kv_len, const int* slots, const float* row_stats, float* weights, int n_slots, int places, int n_seqs,
-                             int max_kv, int n_heads, int n_kv, int head_dim, int page_size, int n_pages, float scale, int chunk_rows, int n_chunks,
+                             int max_kv, int n_heads, int n_kv, int head_dim, int page_size, int n_pages, float scale, int total_tokens, int q_bound,
                              float* ws, hipStream_t stream) {
-    if (n_seqs <= 0 || max_kv <= 0 || n_chunks <= 0) return 0;
+    if (n_seqs <= 0 || max_kv <= 0 || total_tokens <= 0 || q_bound <= 0) return 0;
     if (!sia_weigh_f32_takes(head_dim) || q_row_stride % 4 || ((uintptr_t)q | (uintptr_t)k_pages) % 16 || n_kv <= 0 || n_heads % n_kv || page_size <= 0 ||
-        n_kv > 65535 || n_seqs > 65535 || n_chunks > 65535 || places < max_kv || table_width <= 0 || n_pages <= 0 || n_slots <= 0 || chunk_rows <= 0 ||
-        (n_chunks > n_seqs && !ws))
+        n_seqs > 65535 || places < max_kv || table_width <= 0 || n_pages <= 0 || n_slots <= 0 || (long long)q_bound * (n_heads / n_kv) > 0x7fffff00)
         return SIA_BAD_ARGUMENT;
-    const Weighed w{weights, slots, nullptr, n_slots, places, max_kv};
+    const Cut cut = cut_f32(total_tokens, q_bound, n_seqs, max_kv, n_heads, n_kv);
+    const int blocks = (max_kv + F32_KEYS - 1) / F32_KEYS;
+    if (cut.most_work > 65535 || blocks > 65535 || (cut.floats && !ws)) return SIA_BAD_ARGUMENT;
+    const Weighed w{weights, slots, nullptr, n_slots, places, 0};
     const int most_keys = (int)min((long long)max_kv, (long long)table_width * page_size);
-    float* parts = n_chunks > n_seqs ? ws : nullptr;
+    float* parts = cut.floats ? ws : nullptr;
 #define LAUNCH(DP)                                                                                                                          \
-    hipLaunchKernelGGL(weigh_f32_kernel<DP>, dim3((max_kv + F32_KEYS - 1) / F32_KEYS, n_kv, n_chunks), dim3(F32_WAVES * SIA_WAVE), 0, stream, q, \
-                       q_row_stride, k_pages, block_table, table_width, cu_q, kv_len, row_stats, n_heads, n_kv, head_dim, page_size, n_pages,  \
-                       scale, n_seqs, chunk_rows, most_keys, parts, w)
+    hipLaunchKernelGGL(weigh_f32_kernel<DP>, dim3(n_kv, cut.most_work, n_seqs), dim3(F32_WAVES * SIA_WAVE), 0, stream, q, q_row_stride,       \
+                       k_pages, block_table, table_width, cu_q, kv_len, row_stats, n_heads, n_kv, head_dim, page_size, n_pages, scale,       \
+                       cut.chunk_rows, most_keys, parts, w)
     if (head_dim <= 32) LAUNCH(32);
     else if (head_dim <= 64) LAUNCH(64);
     else LAUNCH(128);
 #undef LAUNCH
     if (parts)
-        hipLaunchKernelGGL(weigh_runs_add_kernel<F32_KEYS>, dim3((max_kv + ADD_THREADS - 1) / ADD_THREADS, n_kv, n_seqs), dim3(ADD_THREADS), 0, stream,
-                           parts, cu_q, kv_len, n_heads, n_kv, 0, chunk_rows, most_keys, w);
+        hipLaunchKernelGGL(weigh_add_kernel<F32_KEYS>, dim3(n_kv, blocks, n_seqs), dim3(F32_KEYS), 0, stream, parts, cu_q, kv_len, n_heads, n_kv, 0,
+                           cut.chunk_rows, most_keys, cut.most_work, w);
     return SIA_LAUNCH_CHECK();
 }

@@ -187,73 +187,165 @@ __global__ __launch_bounds__(JOIN_THREADS) void weighed_join_kernel(
 // ---------------------------------------------------------------------------------------------------
 constexpr int RUN_WAVES = 4, WAVE_BLOCKS = 4, WAVE_KEYS = 16 * WAVE_BLOCKS, RUN_KEYS = RUN_WAVES * WAVE_KEYS;
 
-// grid (blocks of RUN_KEYS keys, key/value heads, chunks of chunk_rows rows of the sequences one after the other); a wave holds its 64 keys as
-// operands and walks the rows 16 at a time.  parts: [chunk][key/value head][row_keys], or null where every sequence has one chunk.
-__global__ __launch_bounds__(RUN_WAVES* SIA_WAVE) void weigh_runs_kernel(
+// grid (key/value heads, pieces of work of a run, runs): workgroups go to the chip's dies in turn, so that with 8 key/value heads a die reads
+// one head's keys and queries.  A wave holds its 64 keys as operands; the rows come through LDS 32 at a time, two stages of it, the next tile's loads under way while one is computed.  (Read from memory as
+// operands, 16 rows of 16 bytes a lane, every lane is an access of its own to the first-level cache: four times as many, and what bound it.)
+// parts: [run][piece of work][key/value head][RUN_KEYS], or null where every block has one chunk.
+constexpr int TILE_ROWS = 32, PIECES = HD / 8, ROW_STRIDE = HD + ((HD / 16) % 2 == 0 ? 16 : 0);      // as the prefill kernel's key rows
+constexpr int RUN_THREADS = RUN_WAVES * SIA_WAVE, PER_THREAD = (TILE_ROWS * PIECES + RUN_THREADS - 1) / RUN_THREADS;
+typedef uint32_t piece_t __attribute__((ext_vector_type(4)));      // a plain 16-byte register value
+
+// A thread's part of a tile of rows: pieces of q, and (of the first 32 threads) a row's statistic and place.
+struct RowTile {
+    piece_t q[PER_THREAD];
+    float stat;
+    int place;
+};
+
+// Lane l of every wave goes with row l % 32 of the tiles; the threads that load the row's pieces ask it for where the row lies.
+struct RowWalk {
+    Column own;
+    int by_token, by_head, last_token, row_end, start, group, n_heads;
+    unsigned stride;      // 16-byte pieces from a token's row to the next
+    const bf16_t* q;      // the row of the chunk's first token, at the group's first head
+    const float* stats;
+};
+
+__device__ __forceinline__ void fetch_rows(RowTile& t, RowWalk& w) {
+    const int token = min(w.own.token, w.last_token);      // behind the last row: some row of the last token, with weights of 0
+    const unsigned at = (unsigned)token * w.stride + w.own.head * PIECES;
+    const float stat = w.stats[(size_t)token * w.n_heads + w.own.head];
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i) {
+        const int c = min((int)threadIdx.x + i * RUN_THREADS, TILE_ROWS * PIECES - 1);
+        t.q[i] = reinterpret_cast<const piece_t*>(w.q)[(size_t)(unsigned)__shfl((int)at, c / PIECES, SIA_WAVE) + c % PIECES];
+    }
+    t.stat = w.own.row < w.row_end ? stat : INFINITY;
+    t.place = w.start + token;
+    w.own.next<TILE_ROWS>(w.by_token, w.by_head, w.group);
+}
+
+__device__ __forceinline__ void store_rows(const RowTile& t, bf16_t* __restrict__ rows, float* __restrict__ stats, int* __restrict__ places) {
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i) {
+        const int c = threadIdx.x + i * RUN_THREADS;
+        if (TILE_ROWS * PIECES % RUN_THREADS == 0 || c < TILE_ROWS * PIECES)
+            *reinterpret_cast<piece_t*>(rows + c / PIECES * ROW_STRIDE + c % PIECES * 8) = t.q[i];
+    }
+    if (threadIdx.x < TILE_ROWS) {
+        stats[threadIdx.x] = t.stat;
+        places[threadIdx.x] = t.place;
+    }
+}
+
+// A tile's rows against the wave's keys, which are k0 .. k0 + 63 (k0 the same in all lanes).
+__device__ __forceinline__ void weigh_rows(floatx4 (&sum)[WAVE_BLOCKS], const bf16x8 (&kf)[WAVE_BLOCKS][KSTEPS], const bf16_t* __restrict__ rows,
+                                           const float* __restrict__ stats, const int* __restrict__ places, int k0, float scale) {
+    constexpr int HALVES = TILE_ROWS / 16;
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    int place[HALVES];
+    float stat[HALVES];
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) {
+        place[h] = places[h * 16 + r];
+        stat[h] = stats[h * 16 + r];
+    }
+    if (__builtin_amdgcn_readlane(place[HALVES - 1], 15) < k0) return;      // none of the rows sees one of the wave's keys: places rise with the rows
+    floatx4 s[HALVES][WAVE_BLOCKS];
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) {
+#pragma unroll
+        for (int v = 0; v < WAVE_BLOCKS; ++v) s[h][v] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ++ks) {
+            // (beyond HD: some elements of the row once more, which meet zeros of the keys)
+            const bf16x8 x = load8(rows + (h * 16 + r) * ROW_STRIDE + (HD % 32 == 0 || ks < KSTEPS - 1 ? ks * 32 + g * 8 : min(ks * 32 + g * 8, HD - 8)));
+#pragma unroll
+            for (int v = 0; v < WAVE_BLOCKS; ++v) s[h][v] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[v][ks], x, s[h][v], 0, 0, 0);
+        }
+    }
+    const bool whole = __builtin_amdgcn_readfirstlane(place[0]) >= k0 + WAVE_KEYS - 1;
+    if (!whole) {
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+            for (int v = 0; v < WAVE_BLOCKS; ++v)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[h][v][i] = k0 + v * 16 + g * 4 + i <= place[h] ? s[h][v][i] : -INFINITY;
+    }
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+        for (int v = 0; v < WAVE_BLOCKS; ++v)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[v][i] += fast_exp2(fmaf(s[h][v][i], scale, -stat[h]));
+}
+
+__global__ __launch_bounds__(RUN_THREADS) void weigh_runs_kernel(
     const bf16_t* __restrict__ q, int q_row_stride, const bf16_t* __restrict__ kp, const int* __restrict__ block_table, int table_width,
     const int* __restrict__ cu_q, const int* __restrict__ kv_len, const float* __restrict__ row_stats, int n_heads, int n_kv, int ps_log2,
-    float scale, int seq_begin, int seq_end, int chunk_rows, int most_keys, float* __restrict__ parts, const Weighed w) {
-    const int hk = blockIdx.y, group = n_heads / n_kv, key0 = blockIdx.x * RUN_KEYS;
-    Run run;
-    if (!find_run(run, blockIdx.z, cu_q, kv_len, seq_begin, seq_end, group, chunk_rows, most_keys)) return;
-    if (key0 >= run.length || !chunk_sees(run.row_end, group, run.start, key0)) return;
-    const int wave = threadIdx.x / SIA_WAVE, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const int k0 = key0 + wave * WAVE_KEYS;
-    if (k0 >= run.length) return;
+    float scale, int seq_begin, int chunk_rows, int most_keys, float* __restrict__ parts, const Weighed w) {
+    __shared__ __attribute__((aligned(16))) bf16_t rows_s[2][TILE_ROWS * ROW_STRIDE];
+    __shared__ float stat_s[2][TILE_ROWS];
+    __shared__ int place_s[2][TILE_ROWS];
+    const int hk = blockIdx.x, group = n_heads / n_kv;
+    Work run;
+    if (!find_work<RUN_KEYS>(run, blockIdx.y, seq_begin + blockIdx.z, cu_q, kv_len, group, chunk_rows, most_keys)) return;      // the whole workgroup
+    float* const part = parts ? parts + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * n_kv + hk) * RUN_KEYS : nullptr;
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+    const int k0 = __builtin_amdgcn_readfirstlane(run.key0 + tid / SIA_WAVE * WAVE_KEYS);
     const int* table = block_table + (size_t)run.seq * table_width;
     scale *= LOG2E;
 
+    const int row_first = run.row_begin;
+    RowWalk walk;
+    walk.by_token = TILE_ROWS / group;
+    walk.by_head = TILE_ROWS - walk.by_token * group;
+    walk.last_token = max(run.row_end - 1, 0) / group;
+    walk.row_end = run.row_end;
+    walk.start = run.start;
+    walk.group = group;
+    walk.n_heads = n_heads;
+    walk.own.begin(row_first + tid % TILE_ROWS, group);
+    const int token_first = min(row_first / group, walk.last_token);      // tokens from here on, so that a piece's index stays small
+    walk.own.token -= token_first;
+    walk.last_token -= token_first;
+    walk.start += token_first;
+    walk.stride = q_row_stride / 8;
+    walk.q = q + (size_t)(run.q_begin + token_first) * q_row_stride + hk * group * HD;
+    walk.stats = row_stats + (size_t)(run.q_begin + token_first) * n_heads + hk * group;
+    RowTile a, b;
+    fetch_rows(a, walk);
+    fetch_rows(b, walk);
     floatx4 sum[WAVE_BLOCKS];
     bf16x8 kf[WAVE_BLOCKS][KSTEPS];
 #pragma unroll
-    for (int b = 0; b < WAVE_BLOCKS; ++b) {
-        sum[b] = floatx4{0.f, 0.f, 0.f, 0.f};
-        const int key = min(k0 + b * 16 + r, run.length - 1);
+    for (int v = 0; v < WAVE_BLOCKS; ++v) {
+        sum[v] = floatx4{0.f, 0.f, 0.f, 0.f};
+        const int key = min(k0 + v * 16 + r, run.length - 1);
         const int page = max(table[key >> ps_log2], 0);
-        load_q(kf[b], kp + (((size_t)page * n_kv + hk) * (1 << ps_log2) + (key & ((1 << ps_log2) - 1))) * HD, g);
-    }
-    // from the first row that sees the wave's first key on
-    const int row_first = max(run.chunk * chunk_rows, max(0, k0 - run.start) * group), by_token = 16 / group, by_head = 16 - by_token * group;
-    const int last_token = (run.row_end - 1) / group;
-    Column col;
-    col.begin(row_first + r, group);
-    auto fetch = [&](bf16x8 (&qf)[KSTEPS], float& stat, int& place) {
-        const int t = min(col.token, last_token);       // behind the last row: some row of the last token, with weights of 0
-        const size_t at = (size_t)(run.q_begin + t);
-        load_q(qf, q + at * q_row_stride + (hk * group + col.head) * HD, g);
-        stat = col.row < run.row_end ? row_stats[at * n_heads + hk * group + col.head] : INFINITY;
-        place = run.start + t;
-        col.next(by_token, by_head, group);
-    };
-    auto compute = [&](const bf16x8 (&qf)[KSTEPS], float stat, int place) {
-        floatx4 s[WAVE_BLOCKS];
+        const bf16_t* row = kp + (((size_t)page * n_kv + hk) * (1 << ps_log2) + (key & ((1 << ps_log2) - 1))) * HD;
 #pragma unroll
-        for (int b = 0; b < WAVE_BLOCKS; ++b) {
-            s[b] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int ks = 0; ks < KSTEPS; ++ks) s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[b][ks], qf[ks], s[b], 0, 0, 0);
+        for (int ks = 0; ks < KSTEPS; ++ks) {
+            const int d0 = ks * 32 + g * 8;
+            kf[v][ks] = load8(row + (HD % 32 == 0 || ks < KSTEPS - 1 ? d0 : min(d0, HD - 8)));
+            if (HD % 32 != 0 && ks == KSTEPS - 1 && d0 >= HD) kf[v][ks] = zero8();
         }
-        const bool whole = __all(k0 + WAVE_KEYS - 1 <= place);
-#pragma unroll
-        for (int b = 0; b < WAVE_BLOCKS; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float p = fast_exp2(fmaf(s[b][i], scale, -stat));
-                sum[b][i] += whole || k0 + b * 16 + g * 4 + i <= place ? p : 0.f;
-            }
-    };
-    bf16x8 qa[KSTEPS], qb[KSTEPS];
-    float sa, sb;
-    int pa, pb;
-    if (row_first < run.row_end) fetch(qa, sa, pa);
-    for (int row0 = row_first; row0 < run.row_end; row0 += 32) {      // the next 16 rows on their way while these are computed
-        fetch(qb, sb, pb);
-        compute(qa, sa, pa);
-        if (row0 + 16 >= run.row_end) break;
-        fetch(qa, sa, pa);
-        compute(qb, sb, pb);
     }
-    leave_sums(sum, k0, run, parts ? parts + ((size_t)blockIdx.z * n_kv + hk) * w.row_keys : nullptr, w, n_kv, hk);
+    const bool live = k0 < run.length;
+    store_rows(a, rows_s[0], stat_s[0], place_s[0]);
+    __syncthreads();
+    for (int row0 = row_first; row0 < run.row_end; row0 += 2 * TILE_ROWS) {
+        fetch_rows(a, walk);
+        if (live) weigh_rows(sum, kf, rows_s[0], stat_s[0], place_s[0], k0, scale);
+        store_rows(b, rows_s[1], stat_s[1], place_s[1]);
+        __syncthreads();
+        fetch_rows(b, walk);
+        if (live && row0 + TILE_ROWS < run.row_end) weigh_rows(sum, kf, rows_s[1], stat_s[1], place_s[1], k0, scale);
+        store_rows(a, rows_s[0], stat_s[0], place_s[0]);
+        __syncthreads();
+    }
+    if (live) leave_sums(sum, k0, run, part, w, n_kv, hk);
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -310,37 +402,38 @@ SIA_EXPORT int sia_attn_weighed_decode(const void* q, int q_row_stride, const vo
     return SIA_LAUNCH_CHECK();
 }
 
-// Rows of a key/value head that one workgroup walks: enough workgroups to fill the chip several times over, none with so few rows that its keys'
-// loads count.  blocks: of RUN_KEYS keys, of the longest sequence.
-SIA_EXPORT int sia_weigh_runs_chunk(int total_rows, int n_kv, int max_kv) {
-    const long long blocks = ((long long)max_kv + RUN_KEYS - 1) / RUN_KEYS;
-    const long long rows = (long long)total_rows * n_kv * blocks / 2048;
-    return (int)(rows < 256 ? 256 : (rows + 63) / 64 * 64);
+// How the runs of a launch are cut.  Two workgroups are on a compute unit at a time: 512 in all.
+static Cut cut_of(int total_tokens, int q_bound, int n_runs, int max_kv, int n_heads, int n_kv) {
+    return cut_runs(total_tokens, q_bound, n_runs, max_kv, n_heads / n_kv, n_kv, RUN_KEYS, 64, 512);
 }
 
-// Floats of the workspace for n_chunks chunks in all (0: every sequence has one).
-SIA_EXPORT long long sia_weigh_runs_workspace(int n_chunks, int n_runs, int n_kv, int max_kv) {
-    return n_chunks <= n_runs ? 0 : (long long)n_chunks * n_kv * row_keys_of(max_kv);
+// Floats of sia_weigh_runs' workspace (0: none).
+SIA_EXPORT long long sia_weigh_runs_workspace(int total_tokens, int q_bound, int n_runs, int max_kv, int n_heads, int n_kv) {
+    if (total_tokens <= 0 || q_bound <= 0 || n_runs <= 0 || max_kv <= 0 || n_kv <= 0 || n_heads % n_kv) return 0;
+    return cut_of(total_tokens, q_bound, n_runs, max_kv, n_heads, n_kv).floats;
 }
 
-// Sequences seq_begin .. seq_end-1, none longer than max_kv; n_chunks: the sum over them of ceil(tokens * n_heads / n_kv / chunk_rows).
+// Sequences seq_begin .. seq_end-1, total_tokens tokens in all, none with more than q_bound tokens and max_kv places.
 SIA_EXPORT int sia_weigh_runs(const void* q, int q_row_stride, const void* k_pages, const int* block_table, int table_width, const int* cu_q,
-                              const int* kv_len, const float* row_stats, float* ws, int seq_begin, int seq_end, int n_heads, int n_kv,
-                              int page_size, float scale, int chunk_rows, int n_chunks, int max_kv, float* weights, const int* slots, int n_slots,
-                              int places, hipStream_t stream) {
-    if (seq_end <= seq_begin || n_chunks <= 0) return 0;
+                              const int* kv_len, const float* row_stats, float* ws, int seq_begin, int seq_end, int total_tokens, int q_bound, int n_heads,
+                              int n_kv, int page_size, float scale, int max_kv, float* weights, const int* slots, int n_slots, int places,
+                              hipStream_t stream) {
+    if (seq_end <= seq_begin || total_tokens <= 0 || q_bound <= 0) return 0;
     const int ps_log2 = log2_of(page_size), n_runs = seq_end - seq_begin;
-    if (ps_log2 < 3 || n_kv <= 0 || n_heads % n_kv || n_kv > 65535 || n_chunks > 65535 || n_runs > 65535 || q_row_stride % 8 || table_width <= 0 || max_kv <= 0 || places < max_kv ||
-        n_slots <= 0 || chunk_rows <= 0 || !row_stats || !weights || (n_chunks > n_runs && !ws))
+    if (ps_log2 < 3 || n_kv <= 0 || n_heads % n_kv || n_runs > 65535 || q_row_stride % 8 || table_width <= 0 || max_kv <= 0 || places < max_kv ||
+        n_slots <= 0 || !row_stats || !weights || (long long)q_bound * (n_heads / n_kv) > 0x7fffff00)
         return SIA_BAD_ARGUMENT;
-    const Weighed w{weights, slots, nullptr, n_slots, places, (int)row_keys_of(max_kv)};
+    const Cut cut = cut_of(total_tokens, q_bound, n_runs, max_kv, n_heads, n_kv);
+    const int blocks = (max_kv + RUN_KEYS - 1) / RUN_KEYS;
+    if (cut.most_work > 65535 || blocks > 65535 || (cut.floats && !ws)) return SIA_BAD_ARGUMENT;
+    const Weighed w{weights, slots, nullptr, n_slots, places, 0};
     const int most_keys = (int)min((long long)max_kv, (long long)table_width << ps_log2);
-    float* parts = n_chunks > n_runs ? ws : nullptr;
-    hipLaunchKernelGGL(weigh_runs_kernel, dim3((max_kv + RUN_KEYS - 1) / RUN_KEYS, n_kv, n_chunks), dim3(RUN_WAVES * SIA_WAVE), 0, stream,
-                       (const bf16_t*)q, q_row_stride, (const bf16_t*)k_pages, block_table, table_width, cu_q, kv_len, row_stats, n_heads, n_kv,
-                       ps_log2, scale, seq_begin, seq_end, chunk_rows, most_keys, parts, w);
+    float* parts = cut.floats ? ws : nullptr;
+    hipLaunchKernelGGL(weigh_runs_kernel, dim3(n_kv, cut.most_work, n_runs), dim3(RUN_THREADS), 0, stream, (const bf16_t*)q, q_row_stride,
+                       (const bf16_t*)k_pages, block_table, table_width, cu_q, kv_len, row_stats, n_heads, n_kv, ps_log2, scale, seq_begin,
+                       cut.chunk_rows, most_keys, parts, w);
     if (parts)
-        hipLaunchKernelGGL(weigh_runs_add_kernel<RUN_KEYS>, dim3((max_kv + ADD_THREADS - 1) / ADD_THREADS, n_kv, n_runs), dim3(ADD_THREADS), 0, stream,
-                           parts, cu_q, kv_len, n_heads, n_kv, seq_begin, chunk_rows, most_keys, w);
+        hipLaunchKernelGGL(weigh_add_kernel<RUN_KEYS>, dim3(n_kv, blocks, n_runs), dim3(RUN_KEYS), 0, stream, parts, cu_q, kv_len, n_heads, n_kv,
+                           seq_begin, cut.chunk_rows, most_keys, cut.most_work, w);
     return SIA_LAUNCH_CHECK();
 }

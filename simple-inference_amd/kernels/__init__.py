@@ -116,8 +116,7 @@ _SIGNATURES = {
     "sia_attention_f32_stats": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
                                 _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_ptr, _c_ptr],
     "sia_weigh_f32_takes": [_c_int],
-    "sia_weigh_f32_chunk": [_c_int, _c_int, _c_int],
-    "sia_weigh_f32_workspace": [_c_int, _c_int, _c_int, _c_int],
+    "sia_weigh_f32_workspace": [_c_int] * 6,
     "sia_weigh_f32": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
                       _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
     "sia_rope_axes_max": [],
@@ -241,10 +240,9 @@ _WEIGHED_SIGNATURES = {
     "sia_attn_weighed_decode_workspace": [_c_int, _c_int, _c_int],
     "sia_attn_weighed_decode": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int,
                                 _c_int, _c_float, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
-    "sia_weigh_runs_chunk": [_c_int, _c_int, _c_int],
-    "sia_weigh_runs_workspace": [_c_int, _c_int, _c_int, _c_int],
+    "sia_weigh_runs_workspace": [_c_int] * 6,
     "sia_weigh_runs": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int,
-                       _c_float, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
+                       _c_int, _c_int, _c_float, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
 }
 
 
@@ -2108,15 +2106,13 @@ class HipKernels:
                 _ptr(ctx.positions), _ptr(out), n, ctx.n_decode_seqs, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim, value_dim, page,
                 float(scale), _ptr(sinks), _ptr(stats), stream), "attention_f32_stats")
             if self.core.sia_weigh_f32_takes(head_dim) and width % 4 == 0 and _in_pieces(qkv, cache.k_pages):
-                group = n_heads // n_kv_heads
-                chunk = self.core.sia_weigh_f32_chunk(n * group, n_kv_heads, max_kv)
-                chunks = sum(-(-q * group // chunk) for q in ctx.q_lens)
-                floats = self.core.sia_weigh_f32_workspace(chunks, ctx.n_seqs, n_kv_heads, max_kv)
+                q_bound = max(ctx.q_lens)
+                floats = self.core.sia_weigh_f32_workspace(n, q_bound, ctx.n_seqs, max_kv, n_heads, n_kv_heads)
                 ws = torch.empty((floats,), dtype=torch.float32, device=qkv.device) if floats else None
                 self._check(self.core.sia_weigh_f32(
                     _ptr(qkv), width, _ptr(cache.k_pages), _ptr(table), table.shape[1], _ptr(ctx.cu_q), _ptr(ctx.kv_len),
                     _ptr(ctx.state_slots), _ptr(stats), _ptr(weights), *places, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim, page,
-                    pages, float(scale), chunk, chunks, _ptr(ws), stream), "weigh_f32")
+                    pages, float(scale), n, q_bound, _ptr(ws), stream), "weigh_f32")
                 return out
         else:
             self._check(self.core.sia_attention_generic_stats(
@@ -2148,14 +2144,12 @@ class HipKernels:
             _ptr(qkv), qkv.shape[1], _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(table), table.shape[1], _ptr(ctx.cu_q),
             _ptr(ctx.kv_len), _ptr(out), n_dec, ctx.n_seqs, *tiles, q_bound, kv_bound, n_heads, n_kv, page, scale, _ptr(sinks),
             _ptr(stats), stream), "attn_prefill_stats")
-        group = n_heads // n_kv
-        chunk = lib.sia_weigh_runs_chunk(sum(ctx.q_lens[n_dec:]) * group, n_kv, kv_bound)
-        chunks, runs = sum(-(-q * group // chunk) for q in ctx.q_lens[n_dec:]), ctx.n_seqs - n_dec
-        floats = lib.sia_weigh_runs_workspace(chunks, runs, n_kv, kv_bound)
+        n_runs, tokens = ctx.n_seqs - n_dec, ctx.n_tokens - n_dec
+        floats = lib.sia_weigh_runs_workspace(tokens, q_bound, n_runs, kv_bound, n_heads, n_kv)
         ws = torch.empty((floats,), dtype=torch.float32, device=device) if floats else None
         self._check(lib.sia_weigh_runs(
             _ptr(qkv), qkv.shape[1], _ptr(cache.k_pages), _ptr(table), table.shape[1], _ptr(ctx.cu_q), _ptr(ctx.kv_len), _ptr(stats),
-            _ptr(ws), n_dec, ctx.n_seqs, n_heads, n_kv, page, scale, chunk, chunks, kv_bound, _ptr(weights), _ptr(ctx.state_slots),
+            _ptr(ws), n_dec, ctx.n_seqs, tokens, q_bound, n_heads, n_kv, page, scale, kv_bound, _ptr(weights), _ptr(ctx.state_slots),
             slots, places, stream), "weigh_runs")
 
     def evict_cache(self, ctx, cache, budget, keep_first=0, keep_last=0):
