@@ -6,10 +6,12 @@
 // keep_last, what is kept below the edge stays where it is; the kept places from the edge on, but for the last, fill the holes below it,
 // both in order; and the last keep_last move up together to the edge, so that the next eviction finds them at the end again.
 //
-// select: a workgroup per (sequence, head): the threshold by radix selection over ordered float keys (11 + 11 + 10 bits), then one ordered
-// walk that lists holes and movers.  move: a workgroup per (sequence, head, slice of a row): nobody else touches these bytes, so that
-// the holes can be filled (their sources lie at or beyond the edge, their targets below it) and then the last moved up, tile after tile,
-// in place.
+// select: a workgroup per (sequence, head), keys of up to 16,384 places in its registers: the threshold by radix selection over ordered float
+// keys (11 + 11 + 10 bits), then holes and movers in order, a wave a stretch of places, so that only the waves' counts cross it.
+// move: a workgroup per (sequence, head, slice of a row): nobody else touches these bytes, so that the holes can be filled (their sources lie
+// at or beyond the edge, their targets below it) and then the last moved up, tile after tile, in place.  Where there are few sequences, movers from
+// beyond the new length, which nothing overwrites, go to further workgroups.
+// What bounds both is latency: a chain of loads, each of whose address is the last one's result, and a barrier or two.
 #include "common.h"
 
 typedef long long ll;
@@ -24,96 +26,148 @@ __device__ __forceinline__ uint32_t order_key(float x) {
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// Sum of v over the threads before this one, and (in total) over all; scratch: SELECT_WAVES ints.
-__device__ __forceinline__ int block_prefix(int v, int* scratch, int& total) {
+// What a wave's value `v` adds up to over the waves before this one, and over all; scratch: SELECT_WAVES ints.
+__device__ __forceinline__ int waves_before(int v, int* scratch, int& total) {
     const int lane = threadIdx.x % SIA_WAVE, wave = threadIdx.x / SIA_WAVE;
-    int s = v;
-#pragma unroll
-    for (int off = 1; off < SIA_WAVE; off *= 2) {
-        const int o = __shfl_up(s, off, SIA_WAVE);
-        if (lane >= off) s += o;
-    }
-    if (lane == SIA_WAVE - 1) scratch[wave] = s;
+    if (lane == 0) scratch[wave] = v;
     __syncthreads();
     int before = 0;
     total = 0;
+#pragma unroll
     for (int w = 0; w < SELECT_WAVES; ++w) {
-        if (w < wave) before += scratch[w];
-        total += scratch[w];
+        const int x = scratch[w];
+        before += w < wave ? x : 0;
+        total += x;
     }
     __syncthreads();
-    return before + s - v;
+    return before;
 }
 
+// HELD: places of a wave's stretch that a lane keeps the keys of (64 HELD places a wave); 0: stretches of any length, read again every time.
+template <int HELD>
 __global__ __launch_bounds__(SELECT_THREADS) void evict_select_kernel(
     const float* __restrict__ weights, const int* __restrict__ slots, const int* __restrict__ kv_len, int n_slots, int places, int max_kv,
     int n_kv, int budget, int keep_first, int keep_last, int max_moves, int* __restrict__ kept, int* __restrict__ lengths,
-    int* __restrict__ from, int* __restrict__ to, int* __restrict__ n_moves) {
+    int* __restrict__ from, int* __restrict__ to, int2* __restrict__ n_moves) {
     __shared__ int bins[BINS];
     __shared__ int scratch[SELECT_WAVES];
-    __shared__ uint32_t found[2];      // the digits so far; how many of the places that match them are still wanted
-    const int hk = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
+    __shared__ uint32_t found[2];      // the largest digit that enough places reach; how many of those that have it are still wanted
+    const int hk = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid % SIA_WAVE, wave = tid / SIA_WAVE;
     const size_t unit = (size_t)seq * n_kv + hk;
     const int slot = slots[seq], length = max(0, min(kv_len[seq], min(max_kv, places)));
     if (hk == 0 && tid == 0) lengths[seq] = min(length, budget);
     int* keep_row = kept + unit * budget;
     if (length <= budget || slot < 0 || slot >= n_slots) {
         for (int i = tid; i < budget; i += SELECT_THREADS) keep_row[i] = i < length ? i : -1;
-        if (tid == 0) n_moves[unit] = -1;      // nothing moves, the last places neither
+        if (tid == 0) n_moves[unit] = make_int2(-1, -1);      // nothing moves, the last places neither
         return;
     }
     const float* w = weights + ((size_t)slot * n_kv + hk) * places;
     const int lo = keep_first, hi = length - keep_last, edge = budget - keep_last;      // between: lo .. hi - 1
     const int wanted = edge - lo;                                                        // fewer than there are
+    from += unit * max_moves;
+    to += unit * max_moves;
+    // the wave's stretch of the places below hi, 64 of them a step
+    const int steps = HELD ? HELD : (hi + SELECT_THREADS - 1) / SELECT_THREADS, begin = wave * steps * SIA_WAVE;
+    uint32_t held[HELD ? HELD : 1];
+    auto load_key = [&](int j) { return j >= lo && j < hi ? order_key(w[j]) : 0u; };      // no place has the key 0: minus infinity has more
+    if constexpr (HELD != 0) {
+        float x[HELD];
+#pragma unroll
+        for (int e = 0; e < HELD; ++e) {
+            const int j = begin + e * SIA_WAVE + lane;
+            x[e] = w[min(j, hi - 1)];
+        }
+#pragma unroll
+        for (int e = 0; e < HELD; ++e) {
+            const int j = begin + e * SIA_WAVE + lane;
+            held[e] = j >= lo && j < hi ? order_key(x[e]) : 0u;
+        }
+    }
+    auto key_at = [&](int e) {
+        if constexpr (HELD != 0) return held[e];
+        else return load_key(begin + e * SIA_WAVE + lane);
+    };
     uint32_t digits = 0;
     int left = wanted;
-    if (wanted > 0)
+    if (wanted > 0) {
+#pragma unroll
         for (int pass = 0; pass < 3; ++pass) {
-            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, size = pass == 2 ? 1024 : 2048;
-            for (int i = tid; i < BINS; i += SELECT_THREADS) bins[i] = 0;
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, mask = pass == 2 ? 1023 : 2047;
+            reinterpret_cast<int2*>(bins)[tid] = make_int2(0, 0);
             __syncthreads();
-            for (int j = lo + tid; j < hi; j += SELECT_THREADS) {
-                const uint32_t key = order_key(w[j]);
-                if (pass == 0 || key >> (pass == 1 ? 21 : 10) == digits) atomicAdd(&bins[(key >> shift) & (size - 1)], 1);
+#pragma unroll
+            for (int e = 0; e < steps; ++e) {
+                const uint32_t key = key_at(e);
+                if (key != 0 && (pass == 0 || key >> (pass == 1 ? 21 : 10) == digits)) atomicAdd(&bins[(key >> shift) & mask], 1);
             }
             __syncthreads();
-            // the largest digit with `left` places at or above it: threads take two bins each from the top
-            const int top = BINS - 1 - 2 * tid, a = bins[top], b = bins[top - 1];
+            // threads take two bins each, from the top
+            const int2 two = reinterpret_cast<const int2*>(bins)[BINS / 2 - 1 - tid];
+            int upto = two.x + two.y;
+#pragma unroll
+            for (int off = 1; off < SIA_WAVE; off *= 2) {
+                const int o = __shfl_up(upto, off, SIA_WAVE);
+                if (lane >= off) upto += o;
+            }
             int total;
-            const int above = block_prefix(a + b, scratch, total);
-            if (above < left && above + a + b >= left) {
-                const bool first = above + a >= left;
-                found[0] = first ? top : top - 1;
-                found[1] = left - (first ? above : above + a);
+            const int above = waves_before(__builtin_amdgcn_readlane(upto, SIA_WAVE - 1), scratch, total) + upto - two.x - two.y;
+            if (above < left && above + two.x + two.y >= left) {
+                const bool upper = above + two.y >= left;
+                found[0] = BINS - 1 - 2 * tid - (upper ? 0 : 1);
+                found[1] = left - (upper ? above : above + two.y);
             }
             __syncthreads();
             digits = digits << (pass == 2 ? 10 : 11) | found[0];
             left = found[1];
-            __syncthreads();
         }
-    // keys above `digits` are kept, and of those equal to it the `left` lowest places
-    int ties = 0, holes = 0, movers = 0;
-    for (int j0 = 0; j0 < hi; j0 += SELECT_THREADS) {
-        const int j = j0 + tid;
-        const uint32_t key = j >= lo && j < hi ? order_key(w[j]) : 0;
-        const bool tie = wanted > 0 && j >= lo && j < hi && key == digits;
-        int total;
-        const int rank = ties + block_prefix(tie, scratch, total);
-        ties += total;
-        const bool keep = j < lo || (j < hi && wanted > 0 && (key > digits || (tie && rank < left)));
-        const bool hole = !keep && j < edge, mover = keep && j >= edge;
-        const int at = block_prefix(hole | (int)mover << 16, scratch, total);
-        if (hole && holes + (at & 0xffff) < max_moves) to[unit * max_moves + holes + (at & 0xffff)] = j;
-        if (mover && movers + (at >> 16) < max_moves) from[unit * max_moves + movers + (at >> 16)] = j;
-        if (keep && j < edge) keep_row[j] = j;
-        holes += total & 0xffff;
-        movers += total >> 16;
+    }
+    // keys above `digits` are kept, and of those equal to it the `left` lowest places (with nothing wanted: none)
+    if (wanted <= 0) digits = 0xffffffffu;
+    int ties = 0;
+#pragma unroll
+    for (int e = 0; e < steps; ++e) ties += __popcll(__ballot(key_at(e) == digits));
+    int total;
+    const int ties_before = wanted > 0 ? waves_before(ties, scratch, total) : 0;
+    const unsigned long long below = (1ull << lane) - 1;
+    // twice over the stretch: first the waves' holes and movers are counted, then they are written in their order
+    int holes = 0, movers = 0, near = 0;
+#pragma unroll
+    for (int round = 0; round < 2; ++round) {
+        ties = ties_before;
+#pragma unroll
+        for (int e = 0; e < steps; ++e) {
+            const int j = begin + e * SIA_WAVE + lane;
+            const uint32_t key = key_at(e);
+            const unsigned long long tied = __ballot(wanted > 0 && key == digits);
+            const bool keep = j < hi && (j < lo || (wanted > 0 && (key > digits || (key == digits && ties + __popcll(tied & below) < left))));
+            const bool hole = !keep && j < edge, mover = keep && j >= edge;
+            const unsigned long long h = __ballot(hole), m = __ballot(mover);
+            ties += __popcll(tied);
+            if (round == 1) {
+                const int at_hole = holes + __popcll(h & below), at_mover = movers + __popcll(m & below);
+                if (hole && at_hole < max_moves) to[at_hole] = j;
+                if (mover && at_mover < max_moves) from[at_mover] = j;
+                if (keep && j < edge) keep_row[j] = j;
+            } else {
+                near += __popcll(__ballot(mover && j < budget));
+            }
+            holes += __popcll(h);
+            movers += __popcll(m);
+        }
+        if (round == 0) {
+            int all_movers, all_near;
+            const int first_hole = waves_before(holes, scratch, total), first_mover = waves_before(movers, scratch, all_movers);
+            waves_before(near, scratch, all_near);
+            holes = first_hole;
+            movers = first_mover;
+            total = min(all_movers, max_moves);
+            if (tid == 0) n_moves[unit] = make_int2(all_near, total);
+        }
     }
     __syncthreads();
-    const int moves = min(movers, max_moves);
-    for (int i = tid; i < moves; i += SELECT_THREADS) keep_row[to[unit * max_moves + i]] = from[unit * max_moves + i];
+    for (int i = tid; i < total; i += SELECT_THREADS) keep_row[to[i]] = from[i];
     for (int i = tid; i < keep_last; i += SELECT_THREADS) keep_row[edge + i] = hi + i;
-    if (tid == 0) n_moves[unit] = moves;
 }
 
 // A sequence's pages and one head of them.
@@ -129,119 +183,155 @@ struct Place {
     }
 };
 
-// Pieces of a key's row: `count` pieces P from `first` on.
+constexpr int MOVE_THREADS = 256;
+
+// A slice of 64 bytes of a key's row: pieces P, a lane a piece, so that a row's lie in neighbouring lanes.
 template <typename P>
 struct KeyPieces {
-    static constexpr int MOST = 4;
+    static constexpr int LANES = 64 / sizeof(P) < 16 ? 64 / sizeof(P) : 16, BATCH = 4;      // lanes a row; rows of a thread at a time
     P* pages;
     Place at;
-    int first, count, row;      // pieces of a row
-    P held[MOST];
+    int first, row;      // the slice's first piece, pieces of a row
+    P held[BATCH];
     __device__ __forceinline__ P* where(int place) const {
         int off;
         const ll head = at.find(place, off);
-        return head < 0 ? nullptr : pages + (head * at.page_size + off) * row + first;
+        const int piece = first + (int)threadIdx.x % LANES;
+        return head < 0 || piece >= row ? nullptr : pages + (head * at.page_size + off) * row + piece;
     }
-    __device__ __forceinline__ bool load(int place) {
+    __device__ __forceinline__ bool load(int b, int place) {
         const P* p = where(place);
-#pragma unroll
-        for (int i = 0; i < MOST; ++i)
-            if (p && i < count) held[i] = p[i];
+        if (p) held[b] = *p;
         return p != nullptr;
     }
-    __device__ __forceinline__ void store(int place) const {
+    __device__ __forceinline__ void store(int b, int place) const {
         P* p = where(place);
-#pragma unroll
-        for (int i = 0; i < MOST; ++i)
-            if (p && i < count) p[i] = held[i];
+        if (p) *p = held[b];
     }
 };
 
-// Dimensions first .. first + count - 1 of a value.
+// Dimensions first .. first + count - 1 of a value, a lane a place.
 template <typename T>
 struct ValueDims {
-    static constexpr int MOST = 16;
+    static constexpr int MOST = 8, LANES = 1, BATCH = 2;
     T* pages;
     Place at;
     int first, count, dim;
-    T held[MOST];
+    T held[BATCH][MOST];
     __device__ __forceinline__ T* where(int place) const {
         int off;
         const ll head = at.find(place, off);
         return head < 0 ? nullptr : pages + (head * dim + first) * at.page_size + off;
     }
-    __device__ __forceinline__ bool load(int place) {
+    __device__ __forceinline__ bool load(int b, int place) {
         const T* p = where(place);
+        if (p) {
 #pragma unroll
-        for (int i = 0; i < MOST; ++i)
-            if (p && i < count) held[i] = p[(size_t)i * at.page_size];
+            for (int i = 0; i < MOST; ++i) held[b][i] = p[(size_t)min(i, count - 1) * at.page_size];
+        }
         return p != nullptr;
     }
-    __device__ __forceinline__ void store(int place) const {
+    __device__ __forceinline__ void store(int b, int place) const {
         T* p = where(place);
+        if (!p) return;
 #pragma unroll
         for (int i = 0; i < MOST; ++i)
-            if (p && i < count) p[(size_t)i * at.page_size] = held[i];
+            if (i < count) p[(size_t)i * at.page_size] = held[b][i];
     }
 };
 
 struct Sums {
+    static constexpr int LANES = 1, BATCH = 2;
     float* row;
-    float held;
-    __device__ __forceinline__ bool load(int place) { held = row[place]; return true; }
-    __device__ __forceinline__ void store(int place) const { row[place] = held; }
+    float held[BATCH];
+    __device__ __forceinline__ bool load(int b, int place) { held[b] = row[place]; return true; }
+    __device__ __forceinline__ void store(int b, int place) const { row[place] = held[b]; }
 };
 
-// Fills the holes, then moves the last places up.  Every thread of the workgroup comes here.
+// Moves begin .. end-1 of the lists: from[i] to to[i].
 template <typename Part>
-__device__ __forceinline__ void move_part(Part part, const int* __restrict__ from, const int* __restrict__ to, int moves, int hi, int edge,
-                                          int keep_last) {
-    for (int i = threadIdx.x; i < moves; i += blockDim.x)
-        if (part.load(from[i])) part.store(to[i]);
-    if (keep_last == 0) return;
-    __syncthreads();      // what lay from the edge on is read
-    for (int i0 = 0; i0 < keep_last; i0 += blockDim.x) {
-        const int i = i0 + threadIdx.x;
-        const bool loaded = i < keep_last && part.load(hi + i);
-        __syncthreads();  // read by all before any is written; the next tile's sources lie beyond this one's targets
-        if (loaded) part.store(edge + i);
+__device__ __forceinline__ void fill(Part& part, const int* __restrict__ from, const int* __restrict__ to, int begin, int end) {
+    constexpr int ROWS = MOVE_THREADS / Part::LANES;
+    for (int i0 = begin + (int)threadIdx.x / Part::LANES; i0 < end; i0 += ROWS * Part::BATCH) {
+        int source[Part::BATCH], target[Part::BATCH];
+        bool loaded[Part::BATCH];
+#pragma unroll
+        for (int b = 0; b < Part::BATCH; ++b) {
+            const int i = min(i0 + b * ROWS, end - 1);
+            source[b] = from[i];
+            target[b] = to[i];
+        }
+#pragma unroll
+        for (int b = 0; b < Part::BATCH; ++b) loaded[b] = i0 + b * ROWS < end && part.load(b, source[b]);
+#pragma unroll
+        for (int b = 0; b < Part::BATCH; ++b)
+            if (loaded[b]) part.store(b, target[b]);
     }
 }
 
+// The last keep_last places from hi on move up to the edge.  Every thread of the workgroup comes here.
+template <typename Part>
+__device__ __forceinline__ void move_up(Part& part, int hi, int edge, int keep_last) {
+    constexpr int ROWS = MOVE_THREADS / Part::LANES;
+    for (int i0 = 0; i0 < keep_last; i0 += ROWS * Part::BATCH) {
+        bool loaded[Part::BATCH];
+        const int mine = i0 + (int)threadIdx.x / Part::LANES;
+#pragma unroll
+        for (int b = 0; b < Part::BATCH; ++b) loaded[b] = mine + b * ROWS < keep_last && part.load(b, hi + mine + b * ROWS);
+        __syncthreads();  // read by all (and what lay from the edge on has filled its holes) before any is written; the next batch's sources lie beyond this one's targets
+#pragma unroll
+        for (int b = 0; b < Part::BATCH; ++b)
+            if (loaded[b]) part.store(b, edge + mine + b * ROWS);
+    }
+}
+
+// A workgroup's share of a part: the first of n_shares has what may be overwritten (all moves, if it is the only one), the others the rest.
+template <typename Part>
+__device__ __forceinline__ void move_part(Part part, int share, int n_shares, const int* __restrict__ from, const int* __restrict__ to, int2 moves,
+                                          int hi, int edge, int keep_last) {
+    if (share > 0) {
+        const int far = moves.y - moves.x, each = (far + n_shares - 2) / (n_shares - 1);
+        fill(part, from, to, moves.x + (share - 1) * each, min(moves.y, moves.x + share * each));
+        return;
+    }
+    fill(part, from, to, 0, n_shares == 1 ? moves.y : moves.x);
+    move_up(part, hi, edge, keep_last);
+}
+
+// grid (sequences x heads, slices of keys and values and one for the sums, shares)
 template <typename T, typename P>
-__global__ __launch_bounds__(256) void evict_move_kernel(
+__global__ __launch_bounds__(MOVE_THREADS) void evict_move_kernel(
     T* k_pages, T* v_pages, float* weights, const int* __restrict__ slots, const int* __restrict__ kv_len,
-    const int* __restrict__ block_table, int table_width, int n_pages, int n_slots, int places, int max_kv, int n_kv, int head_dim, int value_dim,
+    const int* __restrict__ block_table, int table_width, int n_pages, int places, int max_kv, int n_kv, int head_dim, int value_dim,
     int page_size, int page_log2, int budget, int keep_last, int key_slices, int value_slices, int max_moves, const int* __restrict__ from,
-    const int* __restrict__ to, const int* __restrict__ n_moves) {
-    const int hk = blockIdx.x % n_kv, seq = blockIdx.x / n_kv;
+    const int* __restrict__ to, const int2* __restrict__ n_moves) {
+    const int hk = blockIdx.x % n_kv, seq = blockIdx.x / n_kv, share = blockIdx.z, n_shares = gridDim.z;
     const size_t unit = blockIdx.x;
-    const int moves = n_moves[unit];
-    if (moves < 0) return;
+    const int2 moves = n_moves[unit];
     const int length = min(kv_len[seq], min(max_kv, places)), hi = length - keep_last, edge = budget - keep_last;
+    if (moves.y < 0) return;
     from += unit * max_moves;
     to += unit * max_moves;
     const Place at{block_table + (size_t)seq * table_width, table_width, n_pages, n_kv, hk, page_size, page_log2};
     int slice = blockIdx.y;
     if (slice < key_slices) {
         constexpr int PER = sizeof(P) / sizeof(T);
-        const int row = head_dim / PER, first = slice * KeyPieces<P>::MOST;
-        move_part(KeyPieces<P>{(P*)k_pages, at, first, min(KeyPieces<P>::MOST, row - first), row, {}}, from, to, moves, hi, edge, keep_last);
+        move_part(KeyPieces<P>{(P*)k_pages, at, slice * KeyPieces<P>::LANES, head_dim / PER, {}}, share, n_shares, from, to, moves, hi, edge, keep_last);
         return;
     }
     slice -= key_slices;
     if (slice < value_slices) {
         const int first = slice * ValueDims<T>::MOST;
-        move_part(ValueDims<T>{v_pages, at, first, min(ValueDims<T>::MOST, value_dim - first), value_dim, {}}, from, to, moves, hi, edge, keep_last);
+        move_part(ValueDims<T>{v_pages, at, first, min(ValueDims<T>::MOST, value_dim - first), value_dim, {}}, share, n_shares, from, to, moves, hi, edge, keep_last);
         return;
     }
-    move_part(Sums{weights + ((size_t)slots[seq] * n_kv + hk) * places, 0.f}, from, to, moves, hi, edge, keep_last);
+    move_part(Sums{weights + ((size_t)slots[seq] * n_kv + hk) * places, {}}, share, n_shares, from, to, moves, hi, edge, keep_last);
 }
 
 // Ints that sia_evict's workspace holds.
 static int most_moves(int max_kv, int budget, int keep_last) { return max(0, min(budget - keep_last, max_kv - budget)); }
 SIA_EXPORT ll sia_evict_workspace(int n_seqs, int max_kv, int n_kv, int budget, int keep_last) {
-    return (ll)n_seqs * n_kv * (1 + 2LL * most_moves(max_kv, budget, keep_last));
+    return (ll)n_seqs * n_kv * (2 + 2LL * most_moves(max_kv, budget, keep_last));
 }
 
 // kv_len: places of each sequence, none more than max_kv; slots: its row of weights [n_slots][n_kv][places]; kept [n_seqs][n_kv][budget]:
@@ -257,21 +347,31 @@ SIA_EXPORT int sia_evict(void* k_pages, void* v_pages, float* weights, const int
         return SIA_BAD_ARGUMENT;
     const int max_moves = most_moves(max_kv, budget, keep_last);
     const ll units = (ll)n_seqs * n_kv;
-    int *n_moves = ws, *from = ws + units, *to = from + units * max_moves;
-    hipLaunchKernelGGL(evict_select_kernel, dim3(n_kv, n_seqs), dim3(SELECT_THREADS), 0, stream, weights, slots, kv_len, n_slots, places, max_kv,
-                       n_kv, budget, keep_first, keep_last, max_moves, kept, lengths, from, to, n_moves);
+    int2* n_moves = reinterpret_cast<int2*>(ws);
+    int *from = ws + 2 * units, *to = from + units * max_moves;
+#define SELECT(HELD)                                                                                                                     \
+    hipLaunchKernelGGL(evict_select_kernel<HELD>, dim3(n_kv, n_seqs), dim3(SELECT_THREADS), 0, stream, weights, slots, kv_len, n_slots, places, \
+                       max_kv, n_kv, budget, keep_first, keep_last, max_moves, kept, lengths, from, to, n_moves)
+    if (max_kv <= 2 * SELECT_THREADS) SELECT(2);
+    else if (max_kv <= 4 * SELECT_THREADS) SELECT(4);
+    else if (max_kv <= 16 * SELECT_THREADS) SELECT(16);
+    else SELECT(0);
+#undef SELECT
     if (max_kv <= budget) return SIA_LAUNCH_CHECK();      // nothing moves anywhere
     int page_log2 = -1;
     for (int b = 0; b < 31; ++b)
         if (page_size == 1 << b) page_log2 = b;
     // the widest piece that divides a key's row
     const int size = dtype == SIA_F32 ? 4 : 2, bytes = head_dim * size, piece = bytes % 16 == 0 && (uintptr_t)k_pages % 16 == 0 ? 16 : size;
-    const int key_slices = (bytes / piece + 3) / 4, value_slices = (value_dim + 15) / 16;
+    const int lanes = min(64 / piece, 16), key_slices = (bytes / piece + lanes - 1) / lanes, value_slices = (value_dim + 7) / 8, slices = key_slices + value_slices + 1;
+    if (slices > 65535) return SIA_BAD_ARGUMENT;
+    // further workgroups for the movers from beyond the new length, where those that there are leave the chip idle and there may be enough of them
+    const ll far = max(0, min(budget - keep_last, max_kv - keep_last - budget)), there = units * slices;
+    const int shares = 1 + (int)min((far + 255) / 256, there >= 1024 ? 0 : 1024 / there);
 #define LAUNCH(T, P)                                                                                                                    \
-    hipLaunchKernelGGL((evict_move_kernel<T, P>), dim3((unsigned)units, key_slices + value_slices + 1), dim3(256), 0, stream, (T*)k_pages, \
-                       (T*)v_pages, weights, slots, kv_len, block_table, table_width, n_pages, n_slots, places, max_kv, n_kv, head_dim, \
+    hipLaunchKernelGGL((evict_move_kernel<T, P>), dim3((unsigned)units, slices, shares), dim3(MOVE_THREADS), 0, stream, (T*)k_pages,     \
+                       (T*)v_pages, weights, slots, kv_len, block_table, table_width, n_pages, places, max_kv, n_kv, head_dim,           \
                        value_dim, page_size, page_log2, budget, keep_last, key_slices, value_slices, max_moves, from, to, n_moves)
-    if (key_slices + value_slices + 1 > 65535) return SIA_BAD_ARGUMENT;
     if (dtype == SIA_F32) {
         if (piece == 16) LAUNCH(float, uint4);
         else LAUNCH(float, float);

@@ -360,8 +360,9 @@ class HipKernels:
         self._attn_libs = {}
         # the short way to the current stream's handle, where this torch has it (a few microseconds less a launch)
         self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self._current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
         self._device_index = torch.device(device).index or 0
-        self._own_device = torch.device("cuda", self._device_index)
+        self._axes_known: Dict[tuple, tuple] = {}       # what ``rope_axes_kv_write`` makes of its plain arguments
         self.use_mfma_attention = True   # tests switch it off to reach the plain kernel in bfloat16
         self.use_skinny_gemm = True      # few-row bfloat16 products by this package's kernel, not the library
         self.fuse_norms = True           # few rows: residual add in the product before a norm, row scale in the one after
@@ -444,6 +445,13 @@ class HipKernels:
             return self._raw_stream(self._device_index)
         return torch.cuda.current_stream(self.device).cuda_stream
 
+    def _stream_here(self):
+        """``_stream()`` for launches that the device's being the current one is not taken for granted of."""
+        current = self._current_device()
+        if current != self._device_index:
+            raise KernelError(f"the kernels run on cuda:{self._device_index}, the current device is cuda:{current}")
+        return self._stream()
+
     def _check(self, code: int, what: str):
         if code != 0:
             if code == 10001:
@@ -451,8 +459,8 @@ class HipKernels:
             raise KernelError(f"{what}: HIP error {code}")
 
     def _want(self, t: torch.Tensor, what: str, dtype=None, shape=None):
-        if not t.is_cuda:
-            raise KernelError(f"{what} must be on the GPU, is on {t.device}")
+        if t.get_device() != self._device_index:
+            raise KernelError(f"{what} must be on the GPU (cuda:{self._device_index}), is on {t.device}")
         if not t.is_contiguous():
             raise KernelError(f"{what} must be contiguous")
         if dtype is not None and t.dtype != dtype:
@@ -1730,6 +1738,30 @@ class HipKernels:
             raise KernelError(f"qkv row of {width} does not hold {n_heads} + 2*{n_kv_written} heads of {head_dim}")
         if n != ctx.n_tokens:
             raise KernelError(f"qkv has {n} rows, the step {ctx.n_tokens} tokens")
+        key = (tuple(sections), head_dim, order, pairing)
+        known = self._axes_known.get(key)
+        if known is None:
+            known = self._axes_known[key] = self._axes(*key)
+        counts, axes, half, cycled, neighbours = known
+        self._want(cos, "cos table", torch.float32)
+        self._want(sin, "sin table", torch.float32)
+        if cos.dim() != 2 or cos.shape[0] < 1 or cos.shape[1] != half or sin.shape != cos.shape:
+            raise KernelError(f"cos and sin tables {tuple(cos.shape)} and {tuple(sin.shape)} do not hold {half} pairs")
+        self._want(rotary_positions, "rotary positions", torch.int32, (axes, n))
+        k = v = table = None
+        page_size = pages = table_width = 0
+        if n_kv_written:
+            k_pages, v_pages, block_table, page_size = cache.k_pages, cache.v_pages, cache.block_table, cache.page_size
+            self._check_pages(k_pages, v_pages, block_table, page_size, n_kv_written, head_dim, qkv.dtype, ctx)
+            k, v, table = k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr()
+            pages, table_width = k_pages.shape[0], block_table.shape[1]
+        self._check(self.core.sia_rope_axes_kv_write(
+            qkv.data_ptr(), width, cos.data_ptr(), sin.data_ptr(), cos.shape[0], rotary_positions.data_ptr(), counts, axes, cycled,
+            ctx.positions.data_ptr(), ctx.seq_of_token.data_ptr(), table, table_width, k, v, pages, n, n_heads, n_kv_written, head_dim,
+            2 * half, neighbours, page_size, _DT[qkv.dtype], self._stream_here()), "rope_axes_kv_write")
+
+    def _axes(self, sections, head_dim, order, pairing):
+        """``rope_axes_kv_write``'s plain arguments, checked, as the kernel takes them."""
         sections, most = tuple(int(c) for c in sections), self.core.sia_rope_axes_max()
         axes, half = len(sections), sum(sections)
         if not 0 < axes <= most or min(sections) < 0 or not 0 < 2 * half <= head_dim:
@@ -1740,25 +1772,7 @@ class HipKernels:
             raise KernelError(f"sections {sections} cannot be dealt in turn: an axis behind the first would have more pairs than turns")
         if pairing not in ("half", "interleaved"):
             raise KernelError(f"pairing must be 'half' or 'interleaved', got {pairing!r}")
-        for t, what in ((cos, "cos table"), (sin, "sin table")):
-            self._want(t, what, torch.float32)
-            if t.dim() != 2 or t.shape[0] < 1 or t.shape[1] != half:
-                raise KernelError(f"{what} {tuple(t.shape)} does not hold {half} pairs")
-        if cos.shape != sin.shape:
-            raise KernelError(f"cos and sin tables differ: {tuple(cos.shape)} and {tuple(sin.shape)}")
-        self._want(rotary_positions, "rotary positions", torch.int32, (axes, n))
-        table = k_pages = v_pages = None
-        page_size = pages = 0
-        if n_kv_written:
-            k_pages, v_pages, table, page_size = cache.k_pages, cache.v_pages, cache.block_table, cache.page_size
-            self._check_pages(k_pages, v_pages, table, page_size, n_kv_written, head_dim, qkv.dtype, ctx)
-            pages = k_pages.shape[0]
-        self._same_device(qkv, cos, sin, rotary_positions, k_pages, v_pages, table)
-        self._check(self.core.sia_rope_axes_kv_write(
-            _ptr(qkv), width, _ptr(cos), _ptr(sin), cos.shape[0], _ptr(rotary_positions), (ctypes.c_int * most)(*sections), axes,
-            int(order == "cycled"), _ptr(ctx.positions), _ptr(ctx.seq_of_token), _ptr(table),
-            table.shape[1] if table is not None else 0, _ptr(k_pages), _ptr(v_pages), pages, n, n_heads, n_kv_written, head_dim, 2 * half,
-            int(pairing == "interleaved"), page_size, _DT[qkv.dtype], self._stream()), "rope_axes_kv_write")
+        return (ctypes.c_int * most)(*sections), axes, half, int(order == "cycled"), int(pairing == "interleaved")
 
     def qkv_to_cache(self, x, w_qkv, n_heads, n_kv_written, head_dim, rotary_dim, cos, sin, ctx, cache,
                      value_dim=None, bias=None, qk_norm=None, page_dim=None, q_temp=None, extra_columns=0,
@@ -1980,9 +1994,9 @@ class HipKernels:
         self._want(k_pages, "key pages", dtype)
         self._want(v_pages, "value pages", dtype)
         pages = k_pages.shape[0]
-        if tuple(k_pages.shape) != (pages, n_kv, page_size, head_dim):
+        if k_pages.shape != (pages, n_kv, page_size, head_dim):
             raise KernelError(f"key pages {tuple(k_pages.shape)} are not [pages, {n_kv}, {page_size}, {head_dim}]")
-        if tuple(v_pages.shape) != (pages, n_kv, value_dim, page_size):
+        if v_pages.shape != (pages, n_kv, value_dim, page_size):
             raise KernelError(f"value pages {tuple(v_pages.shape)} are not [pages, {n_kv}, {value_dim}, {page_size}]")
         self._want(table, "block table", torch.int32)
         if table.dim() != 2 or table.shape[0] != ctx.n_seqs or table.shape[1] * page_size < ctx.max_kv_len:
@@ -2047,12 +2061,6 @@ class HipKernels:
             float(softcap or 0.0), int(keep_first), _DT[qkv.dtype], self._stream()), "attention_generic")
         return out
 
-    def _same_device(self, *tensors):
-        """Raises for tensors that lie on another device than these kernels are launched on."""
-        for t in tensors:
-            if t is not None and t.device != self._own_device:
-                raise KernelError(f"a tensor lies on {t.device}, the kernels run on {self._own_device}")
-
     def _check_weights(self, cache, ctx, n_kv):
         """The sums that a cache keeps beside its keys: ``[slots, n_kv, places]``, room for every place of the step."""
         weights, most = cache.weights, int(max(ctx.kv_bound or 0, ctx.max_kv_len))
@@ -2088,8 +2096,7 @@ class HipKernels:
         if sinks is not None:
             self._want(sinks, "sinks", torch.float32, (n_heads,))
         weights, max_kv = self._check_weights(cache, ctx, n_kv_heads)
-        self._same_device(qkv, cache.k_pages, cache.v_pages, cache.block_table, weights, sinks)
-        out = torch.empty((n, n_heads * value_dim), dtype=qkv.dtype, device=qkv.device)
+        out = qkv.new_empty((n, n_heads * value_dim))
         if not n:
             return out
         table, pages, page = cache.block_table, cache.k_pages.shape[0], cache.page_size
@@ -2098,8 +2105,8 @@ class HipKernels:
                 and _in_pieces(qkv, cache.k_pages, cache.v_pages)):
             self._weighed_mfma(qkv, out, n_heads, n_kv_heads, head_dim, float(scale), ctx, cache, sinks, weights, max_kv)
             return out
-        stats = torch.empty((n, n_heads), dtype=torch.float32, device=qkv.device)
-        stream, places = self._stream(), (weights.shape[0], weights.shape[2])
+        stats = weights.new_empty((n, n_heads))
+        stream, places = self._stream_here(), (weights.shape[0], weights.shape[2])
         if qkv.dtype == torch.float32:
             self._check(self.core.sia_attention_f32_stats(
                 _ptr(qkv), width, _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(table), table.shape[1], _ptr(ctx.seq_of_token),
@@ -2108,7 +2115,7 @@ class HipKernels:
             if self.core.sia_weigh_f32_takes(head_dim) and width % 4 == 0 and _in_pieces(qkv, cache.k_pages):
                 q_bound = max(ctx.q_lens)
                 floats = self.core.sia_weigh_f32_workspace(n, q_bound, ctx.n_seqs, max_kv, n_heads, n_kv_heads)
-                ws = torch.empty((floats,), dtype=torch.float32, device=qkv.device) if floats else None
+                ws = weights.new_empty((floats,)) if floats else None
                 self._check(self.core.sia_weigh_f32(
                     _ptr(qkv), width, _ptr(cache.k_pages), _ptr(table), table.shape[1], _ptr(ctx.cu_q), _ptr(ctx.kv_len),
                     _ptr(ctx.state_slots), _ptr(stats), _ptr(weights), *places, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim, page,
@@ -2127,30 +2134,28 @@ class HipKernels:
 
     def _weighed_mfma(self, qkv, out, n_heads, n_kv, head_dim, scale, ctx, cache, sinks, weights, max_kv):
         """Single tokens by one walk over keys and values, runs by the attention kernel and the scores once more."""
-        lib, n_dec, device = self._attn_lib(head_dim), ctx.n_decode_seqs, qkv.device
-        table, page, stream = cache.block_table, cache.page_size, self._stream()
-        slots, places = weights.shape[0], weights.shape[2]
+        lib, n_dec, page, stream = self._attn_lib(head_dim), ctx.n_decode_seqs, cache.page_size, self._stream_here()
+        (slots, _, places), (table_width, width) = weights.shape, (cache.block_table.shape[1], qkv.shape[1])
+        q, k, v, table = qkv.data_ptr(), cache.k_pages.data_ptr(), cache.v_pages.data_ptr(), cache.block_table.data_ptr()
+        cu_q, kv_len, sums, rows = ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), weights.data_ptr(), ctx.state_slots.data_ptr()
         if n_dec:
-            ws = torch.empty((lib.sia_attn_weighed_decode_workspace(n_dec, n_heads, max_kv),), dtype=torch.float32, device=device)
+            ws = weights.new_empty((lib.sia_attn_weighed_decode_workspace(n_dec, n_heads, max_kv),))
             self._check(lib.sia_attn_weighed_decode(
-                _ptr(qkv), qkv.shape[1], _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(table), table.shape[1], _ptr(ctx.cu_q),
-                _ptr(ctx.kv_len), _ptr(out), _ptr(ws), n_dec, n_heads, n_kv, page, scale, _ptr(sinks), max_kv, _ptr(weights),
-                _ptr(ctx.state_slots), slots, places, stream), "attn_weighed_decode")
+                q, width, k, v, table, table_width, cu_q, kv_len, out.data_ptr(), ws.data_ptr(), n_dec, n_heads, n_kv, page, scale,
+                _ptr(sinks), max_kv, sums, rows, slots, places, stream), "attn_weighed_decode")
         if n_dec >= ctx.n_seqs:
             return
-        stats = torch.empty((ctx.n_tokens, n_heads), dtype=torch.float32, device=device)
+        stats = weights.new_empty((ctx.n_tokens, n_heads))
         tiles, q_bound, kv_bound = self._run_tiles(lib, ctx)
         self._check(lib.sia_attn_prefill_stats(
-            _ptr(qkv), qkv.shape[1], _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(table), table.shape[1], _ptr(ctx.cu_q),
-            _ptr(ctx.kv_len), _ptr(out), n_dec, ctx.n_seqs, *tiles, q_bound, kv_bound, n_heads, n_kv, page, scale, _ptr(sinks),
-            _ptr(stats), stream), "attn_prefill_stats")
-        n_runs, tokens = ctx.n_seqs - n_dec, ctx.n_tokens - n_dec
-        floats = lib.sia_weigh_runs_workspace(tokens, q_bound, n_runs, kv_bound, n_heads, n_kv)
-        ws = torch.empty((floats,), dtype=torch.float32, device=device) if floats else None
+            q, width, k, v, table, table_width, cu_q, kv_len, out.data_ptr(), n_dec, ctx.n_seqs, *tiles, q_bound, kv_bound, n_heads, n_kv,
+            page, scale, _ptr(sinks), stats.data_ptr(), stream), "attn_prefill_stats")
+        tokens = ctx.n_tokens - n_dec
+        floats = lib.sia_weigh_runs_workspace(tokens, q_bound, ctx.n_seqs - n_dec, kv_bound, n_heads, n_kv)
+        ws = weights.new_empty((floats,)) if floats else None
         self._check(lib.sia_weigh_runs(
-            _ptr(qkv), qkv.shape[1], _ptr(cache.k_pages), _ptr(table), table.shape[1], _ptr(ctx.cu_q), _ptr(ctx.kv_len), _ptr(stats),
-            _ptr(ws), n_dec, ctx.n_seqs, tokens, q_bound, n_heads, n_kv, page, scale, kv_bound, _ptr(weights), _ptr(ctx.state_slots),
-            slots, places, stream), "weigh_runs")
+            q, width, k, table, table_width, cu_q, kv_len, stats.data_ptr(), _ptr(ws), n_dec, ctx.n_seqs, tokens, q_bound, n_heads, n_kv,
+            page, scale, kv_bound, sums, rows, slots, places, stream), "weigh_runs")
 
     def evict_cache(self, ctx, cache, budget, keep_first=0, keep_last=0):
         """Drops what got least attention: every sequence of the step with more than ``budget`` places (``ctx.kv_len``) keeps, for
@@ -2172,17 +2177,16 @@ class HipKernels:
         weights, max_kv = self._check_weights(cache, ctx, n_kv)
         if table.shape[1] * cache.page_size < max_kv:
             raise KernelError(f"block table {tuple(table.shape)} does not cover {max_kv} places with pages of {cache.page_size}")
-        self._same_device(k_pages, v_pages, table, weights)
-        n, device = ctx.n_seqs, weights.device
-        kept = torch.empty((n, n_kv, budget), dtype=torch.int32, device=device)
-        lengths = torch.empty((n,), dtype=torch.int32, device=device)
+        n = ctx.n_seqs
+        kept, lengths = ctx.kv_len.new_empty((n, n_kv, budget)), ctx.kv_len.new_empty((n,))
         if not n:
             return kept, lengths
-        ws = torch.empty((self.core.sia_evict_workspace(n, max_kv, n_kv, budget, keep_last),), dtype=torch.int32, device=device)
+        ws = ctx.kv_len.new_empty((self.core.sia_evict_workspace(n, max_kv, n_kv, budget, keep_last),))
         self._check(self.core.sia_evict(
-            _ptr(k_pages), _ptr(v_pages), _ptr(weights), _ptr(ctx.state_slots), _ptr(ctx.kv_len), _ptr(table), table.shape[1],
-            k_pages.shape[0], weights.shape[0], weights.shape[2], n, max_kv, n_kv, head_dim, value_dim, cache.page_size, budget,
-            keep_first, keep_last, _ptr(kept), _ptr(lengths), _ptr(ws), _DT[k_pages.dtype], self._stream()), "evict")
+            k_pages.data_ptr(), v_pages.data_ptr(), weights.data_ptr(), ctx.state_slots.data_ptr(), ctx.kv_len.data_ptr(), table.data_ptr(),
+            table.shape[1], k_pages.shape[0], weights.shape[0], weights.shape[2], n, max_kv, n_kv, head_dim, value_dim, cache.page_size,
+            budget, keep_first, keep_last, kept.data_ptr(), lengths.data_ptr(), ws.data_ptr(), _DT[k_pages.dtype], self._stream_here()),
+            "evict")
         return kept, lengths
 
     @staticmethod
