@@ -122,6 +122,8 @@ ROTATIONS = [
     ([21], [21], 2, 2, 6, (1, 1), "blocks", "interleaved", 4),
     ([130], [130], 2, 2, 256, (64, 0, 64), "blocks", "half", 32),                # an axis without pairs
     ([200, 1, 65], [264, 9, 65], 24, 8, 96, (16, 16, 16), "cycled", "half", 16),
+    ([40], [43], 1, 1, 392, (98, 98), "cycled", "interleaved", 16),              # pieces that fill no wave
+    ([1] * 70, [17 + i for i in range(70)], 4, 4, 192, (40, 20, 20), "blocks", "half", 8),
     ([2100], [2137], 4, 1, 64, (12, 10, 10), "blocks", "half", 16),              # long enough for workgroups of several tokens
 ]
 
