@@ -178,41 +178,6 @@ __global__ __launch_bounds__(DEC_WAVES* SIA_WAVE) void attn_decode_kernel(
 // 128 with 4 splits 3.4 -> 2.0, 27 of 32 of 64, most with one, 2.6 -> 1.8, 3 of 32 of 128 with up to 32 8.0 -> 4.3.)
 constexpr int COMBINE_THREADS = (HD + SIA_WAVE - 1) / SIA_WAVE * SIA_WAVE;
 
-// The states of the first N splits, beyond `last` that one again.
-template <int N>
-__device__ __forceinline__ void load_states(int last, const float* __restrict__ acc_at, const float2* __restrict__ ml, float (&acc)[N],
-                                            float2 (&state)[N]) {
-#pragma unroll
-    for (int s = 0; s < N; ++s) acc[s] = acc_at[(size_t)min(s, last) * HD];
-#pragma unroll
-    for (int s = 0; s < N; ++s) state[s] = ml[min(s, last)];
-}
-
-// merge_splits for one element of up to N splits, with its order of sums.  What is held of splits beyond n_splits may be anything.
-template <int N>
-__device__ __forceinline__ float combine_states(int n_splits, const float (&acc)[N], const float2 (&state)[N], const float* __restrict__ sinks,
-                                                int head) {
-    float mx = -INFINITY;
-#pragma unroll
-    for (int s = 0; s < N; ++s) mx = s < n_splits ? fmaxf(mx, state[s].x) : mx;
-    float o = 0.f, denom = sink_term(sinks, head, mx);
-#pragma unroll
-    for (int s = 0; s < N; ++s) {
-        const float w = fast_exp2(state[s].x - mx), d = __builtin_fmaf(w, state[s].y, denom), a = __builtin_fmaf(w, acc[s], o);
-        denom = s < n_splits ? d : denom;
-        o = s < n_splits ? a : o;
-    }
-    return o * (1.f / denom);
-}
-template <int N>
-__device__ __forceinline__ float combine_all(int n_splits, const float* __restrict__ acc_at, const float2* __restrict__ ml,
-                                             const float* __restrict__ sinks, int head) {
-    float acc[N];
-    float2 state[N];
-    load_states(n_splits - 1, acc_at, ml, acc, state);
-    return combine_states(n_splits, acc, state, sinks, head);
-}
-
 __global__ __launch_bounds__(COMBINE_THREADS) void attn_decode_combine_kernel(
     const float* __restrict__ ws_acc, const float* __restrict__ ws_ml, const int* __restrict__ cu_q,
     const int* __restrict__ kv_len, bf16_t* __restrict__ out, int n_heads, int max_splits, int window, int chunk,

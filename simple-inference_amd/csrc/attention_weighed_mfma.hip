@@ -24,6 +24,18 @@ __device__ __forceinline__ void add_weights(float* __restrict__ row, const float
     }
 }
 
+#ifndef WT
+#define WT 8
+#endif
+// Workgroups of four waves that share one (sequence, key/value head) with n_tiles tiles: the largest power of two that leaves each WEIGHED_TILES.  A
+// function of the sequence's own length only.
+constexpr int WEIGHED_TILES = WT, WEIGHED_MAX_SPLITS = 64;
+__host__ __device__ inline int weighed_splits(int n_tiles) {
+    int s = 1;
+    while (s < WEIGHED_MAX_SPLITS && 2 * s * WEIGHED_TILES <= n_tiles) s *= 2;
+    return s;
+}
+
 // Scores of a tile as they go into the workspace: lane (r, g) holds keys kb + 8 g .. + 7 of column r.
 __device__ __forceinline__ void leave_scores(float* __restrict__ mine, int kb, int g, const floatx4 (&s)[2], float scale) {
     float4* to = reinterpret_cast<float4*>(mine + kb + 8 * g);
@@ -61,7 +73,7 @@ __global__ __launch_bounds__(DEC_WAVES* SIA_WAVE) void weighed_decode_kernel(
             out[((size_t)cu_q[seq] * n_heads + hg * group) * HD + i] = 0;
         return;
     }
-    const int n_tiles = last / TILE + 1, n_splits = min(decode_splits(n_tiles), max_splits);
+    const int n_tiles = last / TILE + 1, n_splits = min(weighed_splits(n_tiles), max_splits);
     if (split >= n_splits) return;
     scale *= LOG2E;  // exponentials are taken as powers of two
     const int hk = hg / kv_share, n_kv = n_groups / kv_share;
@@ -138,48 +150,63 @@ __global__ __launch_bounds__(DEC_WAVES* SIA_WAVE) void weighed_decode_kernel(
     if (row) add_weights(row, w.scores + ((size_t)seq * n_heads + hg * group) * w.row_keys, w.row_keys, stat, group, 0, length, length, threadIdx.x, DEC_WAVES * SIA_WAVE);
 }
 
-// grid (key/value heads, sequences, 1 + chunks of JOIN_KEYS keys): workgroup 0 merges the splits' results, the others make the weights
-// of their keys from the scores, with the rows' statistics made anew from the splits' (a few hundred bytes).
-constexpr int JOIN_KEYS = 512, JOIN_THREADS = 256, JOIN_MOST_HEADS = 256;
-__global__ __launch_bounds__(JOIN_THREADS) void weighed_join_kernel(
+// grid (key/value heads, sequences, query heads of a group + chunks of JOIN_KEYS keys): the first merge the splits' results of a query head
+// each, the others make the weights of their keys from the scores, a thread a key, with the rows' statistics made anew from the splits' (a few hundred
+// bytes).  Latency bounds both: what does not depend on another load's result is asked for first.
+constexpr int JOIN_KEYS = 256, JOIN_MOST_HEADS = 256;
+__global__ __launch_bounds__(JOIN_KEYS) void weighed_join_kernel(
     const float* __restrict__ ws_acc, const float* __restrict__ ws_ml, const int* __restrict__ cu_q, const int* __restrict__ kv_len,
     bf16_t* __restrict__ out, int n_heads, int n_kv, int max_splits, int kv_share, const float* __restrict__ sinks, int most_keys,
     const Weighed w) {
-    const int hk = blockIdx.x, seq = blockIdx.y, chunk = (int)blockIdx.z - 1;
-    const int length = min(kv_len[seq], most_keys), group = n_heads / n_kv;
+    const int hk = blockIdx.x, seq = blockIdx.y, group = n_heads / n_kv, chunk = (int)blockIdx.z - group;
+    const int length = min(kv_len[seq], most_keys);
     if (length <= 0 || chunk * JOIN_KEYS >= length) return;
-    const int n_splits = min(decode_splits((length - 1) / TILE + 1), max_splits);
+    const int n_splits = min(weighed_splits((length - 1) / TILE + 1), max_splits);
     if (n_splits == 1 && (kv_share == 1 || chunk < 0)) return;      // finished by its one workgroup
-    __shared__ float stat[JOIN_MOST_HEADS];
     const size_t base = ((size_t)seq * n_heads + hk * group) * max_splits;
     const float2* const ml = reinterpret_cast<const float2*>(ws_ml) + base;
     if (chunk < 0) {
-        for (int idx = threadIdx.x; idx < group * HD; idx += JOIN_THREADS) {
-            const int c = idx / HD, d = idx % HD, head = hk * group + c;
-            float mx = -INFINITY;
-            for (int s = 0; s < n_splits; ++s) mx = fmaxf(mx, ml[(size_t)c * max_splits + s].x);
-            const float* acc_at = ws_acc + (base + (size_t)c * max_splits) * HD + d;
-            out[((size_t)cu_q[seq] * n_heads + head) * HD + d] = float_to_bf16(merge_splits(n_splits, mx, sink_term(sinks, head, mx), [&](int s, float& a, float& m, float& l) {
-                const float2 state = ml[(size_t)c * max_splits + s];
-                a = acc_at[(size_t)s * HD];
-                m = state.x;
-                l = state.y;
-            }));
-        }
+        const int c = blockIdx.z, head = hk * group + c, d = min((int)threadIdx.x, HD - 1);
+        const float* const acc_at = ws_acc + (base + (size_t)c * max_splits) * HD + d;
+        const float2* const mine = ml + (size_t)c * max_splits;
+        const float o = n_splits <= 8    ? combine_all<8>(n_splits, acc_at, mine, sinks, head)
+                        : n_splits <= 16 ? combine_all<16>(n_splits, acc_at, mine, sinks, head)
+                        : n_splits <= 32 ? combine_all<32>(n_splits, acc_at, mine, sinks, head)
+                                         : combine_all<WEIGHED_MAX_SPLITS>(n_splits, acc_at, mine, sinks, head);
+        if (threadIdx.x < HD) out[((size_t)cu_q[seq] * n_heads + head) * HD + d] = float_to_bf16(o);
         return;
     }
-    for (int c = threadIdx.x; c < group; c += JOIN_THREADS) {
-        float mx = -INFINITY;
-        for (int s = 0; s < n_splits; ++s) mx = fmaxf(mx, ml[(size_t)c * max_splits + s].x);
-        float total = sink_term(sinks, hk * group + c, mx);
-        for (int s = 0; s < n_splits; ++s) total = fmaf(fast_exp2(ml[(size_t)c * max_splits + s].x - mx), ml[(size_t)c * max_splits + s].y, total);
-        stat[c] = mx + log2f(total);
+    __shared__ float stat[JOIN_MOST_HEADS];
+    const int j = min(chunk * JOIN_KEYS + (int)threadIdx.x, length - 1);
+    const float* const scores = w.scores + ((size_t)seq * n_heads + hk * group) * w.row_keys + j;
+    constexpr int AHEAD = 8;
+    float s[AHEAD];
+#pragma unroll
+    for (int c = 0; c < AHEAD; ++c) s[c] = scores[(size_t)min(c, group - 1) * w.row_keys];
+    float* row = weight_row(w, seq, n_kv, hk);
+    const float old = row && j < length - 1 ? row[j] : 0.f;      // the last key is the step's own: its sum begins at zero
+    // statistics: 16 lanes a query head, a split each at a time
+    for (int c0 = threadIdx.x / 16; c0 < (group + JOIN_KEYS / 16 - 1) / (JOIN_KEYS / 16) * (JOIN_KEYS / 16); c0 += JOIN_KEYS / 16) {
+        const int c = min(c0, group - 1), lane = threadIdx.x % 16;
+        float mx = -INFINITY, total = 0.f;
+        for (int s0 = lane; s0 < n_splits; s0 += 16) {
+            const float2 state = ml[(size_t)c * max_splits + s0];
+            const float top = fmaxf(mx, state.x), was = mx == -INFINITY ? 0.f : total * fast_exp2(mx - top);
+            total = state.x == -INFINITY ? was : fmaf(fast_exp2(state.x - top), state.y, was);
+            mx = top;
+        }
+        float top = mx;
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 16));
+        total = row_sum(mx == -INFINITY ? 0.f : total * fast_exp2(mx - top)) + sink_term(sinks, hk * group + c, top);
+        if (lane == 0 && c0 < group) stat[c] = top + log2f(total);
     }
     __syncthreads();
-    float* row = weight_row(w, seq, n_kv, hk);
-    if (row)
-        add_weights(row, w.scores + ((size_t)seq * n_heads + hk * group) * w.row_keys, w.row_keys, stat, group, chunk * JOIN_KEYS,
-                    min(length, (chunk + 1) * JOIN_KEYS), length, threadIdx.x, JOIN_THREADS);
+    float sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < AHEAD; ++c) sum += c < group ? fast_exp2(s[c] - stat[min(c, group - 1)]) : 0.f;
+    for (int c = AHEAD; c < group; ++c) sum += fast_exp2(scores[(size_t)c * w.row_keys] - stat[c]);
+    if (row && chunk * JOIN_KEYS + (int)threadIdx.x < length) row[j] = old + sum;
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -359,7 +386,7 @@ static int log2_of(int v) {
 
 // Floats from one head's scores (or one chunk's sums) to the next for sequences of up to max_kv places: whole tiles.
 static long long row_keys_of(int max_kv) { return ((long long)max_kv + TILE - 1) / TILE * TILE; }
-static int splits_of(int max_kv) { return decode_splits((max_kv + TILE - 1) / TILE); }
+static int splits_of(int max_kv) { return weighed_splits((max_kv + TILE - 1) / TILE); }
 
 // Groups of query heads that share a key/value head: a launch's columns are 16, and the four waves' states lie in 64 KiB.
 static int shares_of(int group) {
@@ -397,7 +424,7 @@ SIA_EXPORT int sia_attn_weighed_decode(const void* q, int q_row_stride, const vo
                        q_row_stride, (const bf16_t*)k_pages, (const bf16_t*)v_pages, block_table, table_width, cu_q, kv_len, acc, ml, (bf16_t*)out,
                        n_heads, n_groups, ps_log2, scale, sinks, max_splits, share, most_keys, w);
     if (max_splits > 1 || share > 1)
-        hipLaunchKernelGGL(weighed_join_kernel, dim3(n_kv, n_seqs, 1 + (max_kv + JOIN_KEYS - 1) / JOIN_KEYS), dim3(JOIN_THREADS), 0, stream, acc, ml,
+        hipLaunchKernelGGL(weighed_join_kernel, dim3(n_kv, n_seqs, n_heads / n_kv + (max_kv + JOIN_KEYS - 1) / JOIN_KEYS), dim3(JOIN_KEYS), 0, stream, acc, ml,
                            cu_q, kv_len, (bf16_t*)out, n_heads, n_kv, max_splits, share, sinks, most_keys, w);
     return SIA_LAUNCH_CHECK();
 }
