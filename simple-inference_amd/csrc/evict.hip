@@ -18,12 +18,26 @@ typedef long long ll;
 #define SELECT_THREADS 1024
 #define SELECT_WAVES (SELECT_THREADS / SIA_WAVE)
 #define BINS 2048
+#define COPIES 4      // of the histogram: weights crowd into few of the first digit's bins, and lanes that meet in one wait for each other
 
 // Larger floats have larger keys; both zeros have the same.
 __device__ __forceinline__ uint32_t order_key(float x) {
     if (x != x) x = -INFINITY;
     const uint32_t u = __float_as_uint(x == 0.f ? 0.f : x);
     return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+// Sum of v over the lanes up to this one, by moves between lanes within the vector unit (a shuffle goes through LDS and takes ten times as long).
+__device__ __forceinline__ int lanes_upto(int v) {
+#define ADD_MOVED(CTRL, ROWS) v += __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false)
+    ADD_MOVED(0x111, 0xf);      // rows of 16 lanes, from 1, 2, 4 and 8 lanes below
+    ADD_MOVED(0x112, 0xf);
+    ADD_MOVED(0x114, 0xf);
+    ADD_MOVED(0x118, 0xf);
+    ADD_MOVED(0x142, 0xa);      // the last lane of rows 0 and 2 to rows 1 and 3, then that of row 1 to rows 2 and 3
+    ADD_MOVED(0x143, 0xc);
+#undef ADD_MOVED
+    return v;
 }
 
 // What a wave's value `v` adds up to over the waves before this one, and over all; scratch: SELECT_WAVES ints.
@@ -49,7 +63,7 @@ __global__ __launch_bounds__(SELECT_THREADS) void evict_select_kernel(
     const float* __restrict__ weights, const int* __restrict__ slots, const int* __restrict__ kv_len, int n_slots, int places, int max_kv,
     int n_kv, int budget, int keep_first, int keep_last, int max_moves, int* __restrict__ kept, int* __restrict__ lengths,
     int* __restrict__ from, int* __restrict__ to, int2* __restrict__ n_moves) {
-    __shared__ int bins[BINS];
+    __shared__ int bins[COPIES][BINS];
     __shared__ int scratch[SELECT_WAVES];
     __shared__ uint32_t found[2];      // the largest digit that enough places reach; how many of those that have it are still wanted
     const int hk = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid % SIA_WAVE, wave = tid / SIA_WAVE;
@@ -94,22 +108,24 @@ __global__ __launch_bounds__(SELECT_THREADS) void evict_select_kernel(
 #pragma unroll
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, mask = pass == 2 ? 1023 : 2047;
-            reinterpret_cast<int2*>(bins)[tid] = make_int2(0, 0);
+#pragma unroll
+            for (int c = 0; c < COPIES; ++c) reinterpret_cast<int2*>(bins[c])[tid] = make_int2(0, 0);
             __syncthreads();
 #pragma unroll
             for (int e = 0; e < steps; ++e) {
                 const uint32_t key = key_at(e);
-                if (key != 0 && (pass == 0 || key >> (pass == 1 ? 21 : 10) == digits)) atomicAdd(&bins[(key >> shift) & mask], 1);
+                if (key != 0 && (pass == 0 || key >> (pass == 1 ? 21 : 10) == digits)) atomicAdd(&bins[lane % COPIES][(key >> shift) & mask], 1);
             }
             __syncthreads();
             // threads take two bins each, from the top
-            const int2 two = reinterpret_cast<const int2*>(bins)[BINS / 2 - 1 - tid];
-            int upto = two.x + two.y;
+            int2 two = make_int2(0, 0);
 #pragma unroll
-            for (int off = 1; off < SIA_WAVE; off *= 2) {
-                const int o = __shfl_up(upto, off, SIA_WAVE);
-                if (lane >= off) upto += o;
+            for (int c = 0; c < COPIES; ++c) {
+                const int2 own = reinterpret_cast<const int2*>(bins[c])[BINS / 2 - 1 - tid];
+                two.x += own.x;
+                two.y += own.y;
             }
+            const int upto = lanes_upto(two.x + two.y);
             int total;
             const int above = waves_before(__builtin_amdgcn_readlane(upto, SIA_WAVE - 1), scratch, total) + upto - two.x - two.y;
             if (above < left && above + two.x + two.y >= left) {
@@ -122,73 +138,105 @@ __global__ __launch_bounds__(SELECT_THREADS) void evict_select_kernel(
             left = found[1];
         }
     }
-    // keys above `digits` are kept, and of those equal to it the `left` lowest places (with nothing wanted: none)
-    if (wanted <= 0) digits = 0xffffffffu;
-    int ties = 0;
+    // keys above `digits` are kept, and of those equal to it the `left` lowest places (with nothing wanted: none of a key that there is not)
+    if (wanted <= 0) digits = 0xffffffffu, left = 0;
+    // A wave's stretch: places below lo, between, beyond hi.  First the waves' counts: of ties, and of what is kept but for ties, below the edge, from
+    // the edge on, and of that below the new length.
+    int ties = 0, stay = 0, beyond = 0, near = 0;      // a lane's own, then the wave's
 #pragma unroll
-    for (int e = 0; e < steps; ++e) ties += __popcll(__ballot(key_at(e) == digits));
+    for (int e = 0; e < steps; ++e) {
+        const int j = begin + e * SIA_WAVE + lane;
+        const uint32_t key = key_at(e);
+        const bool over = key > digits && wanted > 0, tie = key == digits;
+        ties += __popcll(__ballot(tie));
+        stay += (over || j < lo) && j < edge;
+        beyond += over && j >= edge;
+        near += over && j >= edge && j < budget;
+    }
     int total;
-    const int ties_before = wanted > 0 ? waves_before(ties, scratch, total) : 0;
+    const int ties_before = waves_before(ties, scratch, total);
     const unsigned long long below = (1ull << lane) - 1;
-    // twice over the stretch: first the waves' holes and movers are counted, then they are written in their order
-    int holes = 0, movers = 0, near = 0;
-#pragma unroll
-    for (int round = 0; round < 2; ++round) {
-        ties = ties_before;
+    // of the ties, those with fewer than `left` before them: where they lie matters to the counts only if the wave has some of them and some not
+    const int ties_kept = min(max(left - ties_before, 0), ties);
+    if (ties_kept > 0) {
+        int rank = 0;
 #pragma unroll
         for (int e = 0; e < steps; ++e) {
             const int j = begin + e * SIA_WAVE + lane;
-            const uint32_t key = key_at(e);
-            const unsigned long long tied = __ballot(wanted > 0 && key == digits);
-            const bool keep = j < hi && (j < lo || (wanted > 0 && (key > digits || (key == digits && ties + __popcll(tied & below) < left))));
-            const bool hole = !keep && j < edge, mover = keep && j >= edge;
-            const unsigned long long h = __ballot(hole), m = __ballot(mover);
-            ties += __popcll(tied);
-            if (round == 1) {
-                const int at_hole = holes + __popcll(h & below), at_mover = movers + __popcll(m & below);
-                if (hole && at_hole < max_moves) to[at_hole] = j;
-                if (mover && at_mover < max_moves) from[at_mover] = j;
-                if (keep && j < edge) keep_row[j] = j;
-            } else {
-                near += __popcll(__ballot(mover && j < budget));
+            const bool tie = key_at(e) == digits;
+            const unsigned long long tied = __ballot(tie);
+            if (tied) {
+                const bool keep = tie && rank + __popcll(tied & below) < ties_kept;
+                stay += keep && j < edge;
+                beyond += keep && j >= edge;
+                near += keep && j >= edge && j < budget;
+                rank += __popcll(tied);
             }
+        }
+    }
+    // the wave's holes: its places below the edge that nothing stays at
+    const int reach = steps * SIA_WAVE, upper = min(max(edge - begin, 0), reach);
+    const int packed_stay = __builtin_amdgcn_readlane(lanes_upto(stay), SIA_WAVE - 1);
+    int all_movers, all_near;
+    int holes = waves_before(upper - packed_stay, scratch, total);
+    int movers = waves_before(__builtin_amdgcn_readlane(lanes_upto(beyond), SIA_WAVE - 1), scratch, all_movers);
+    waves_before(__builtin_amdgcn_readlane(lanes_upto(near), SIA_WAVE - 1), scratch, all_near);
+    total = min(all_movers, max_moves);
+    if (tid == 0) n_moves[unit] = make_int2(all_near, total);
+    // then the lists, in order
+    int rank = 0;
+#pragma unroll
+    for (int e = 0; e < steps; ++e) {
+        const int j = begin + e * SIA_WAVE + lane;
+        const uint32_t key = key_at(e);
+        bool keep = j < lo || (key > digits && wanted > 0);
+        if (ties_kept > 0) {
+            const unsigned long long tied = __ballot(key == digits);
+            if (tied) {
+                keep |= key == digits && rank + __popcll(tied & below) < ties_kept;
+                rank += __popcll(tied);
+            }
+        }
+        const bool hole = !keep && j < edge, mover = keep && j >= edge;
+        const unsigned long long h = __ballot(hole), m = __ballot(mover);
+        if (h) {
+            const int at = holes + __popcll(h & below);
+            if (hole && at < max_moves) to[at] = j;
             holes += __popcll(h);
+        }
+        if (m) {
+            const int at = movers + __popcll(m & below);
+            if (mover && at < max_moves) from[at] = j;
             movers += __popcll(m);
         }
-        if (round == 0) {
-            int all_movers, all_near;
-            const int first_hole = waves_before(holes, scratch, total), first_mover = waves_before(movers, scratch, all_movers);
-            waves_before(near, scratch, all_near);
-            holes = first_hole;
-            movers = first_mover;
-            total = min(all_movers, max_moves);
-            if (tid == 0) n_moves[unit] = make_int2(all_near, total);
-        }
+        if (keep && j < edge) keep_row[j] = j;
     }
     __syncthreads();
     for (int i = tid; i < total; i += SELECT_THREADS) keep_row[to[i]] = from[i];
     for (int i = tid; i < keep_last; i += SELECT_THREADS) keep_row[edge + i] = hi + i;
 }
 
-// A sequence's pages and one head of them.
+// A sequence's pages and one head of them.  The first entries of its block table lie in LDS: what is moved then waits for one load less.
+constexpr int TABLE_HELD = 1024;
 struct Place {
-    const int* table;
+    const int *table, *held;
     int table_width, n_pages, n_kv, hk, page_size, page_log2;
     // index of (page, head) and the place within; negative: no page
     __device__ __forceinline__ ll find(int place, int& off) const {
         const int index = page_log2 >= 0 ? place >> page_log2 : place / page_size;
         off = page_log2 >= 0 ? place & (page_size - 1) : place % page_size;
-        const int page = index < table_width ? table[index] : -1;
+        const int page = index >= table_width ? -1 : index < TABLE_HELD ? held[index] : table[index];
         return page < 0 || page >= n_pages ? -1 : (ll)page * n_kv + hk;
     }
 };
 
 constexpr int MOVE_THREADS = 256;
+typedef uint32_t piece16 __attribute__((ext_vector_type(4)));      // a plain 16-byte register value
 
-// A slice of 64 bytes of a key's row: pieces P, a lane a piece, so that a row's lie in neighbouring lanes.
+// A slice of a key's row, four pieces P (of 16 bytes, or elements where rows do not lie so): a lane a piece, so that a row's lie in neighbouring lanes.
 template <typename P>
 struct KeyPieces {
-    static constexpr int LANES = 64 / sizeof(P) < 16 ? 64 / sizeof(P) : 16, BATCH = 4;      // lanes a row; rows of a thread at a time
+    static constexpr int LANES = 4, BATCH = 4;      // lanes a row (8: 8 x 2,112 to 2,048 12.7 -> 17.6 us); rows of a thread at a time
     P* pages;
     Place at;
     int first, row;      // the slice's first piece, pieces of a row
@@ -213,7 +261,7 @@ struct KeyPieces {
 // Dimensions first .. first + count - 1 of a value, a lane a place.
 template <typename T>
 struct ValueDims {
-    static constexpr int MOST = 8, LANES = 1, BATCH = 2;
+    static constexpr int MOST = 16, LANES = 1, BATCH = 2;
     T* pages;
     Place at;
     int first, count, dim;
@@ -269,21 +317,23 @@ __device__ __forceinline__ void fill(Part& part, const int* __restrict__ from, c
     }
 }
 
-// The last keep_last places from hi on move up to the edge.  Every thread of the workgroup comes here.
+// A batch of the last places on their way up, from hi + i0 on.
 template <typename Part>
-__device__ __forceinline__ void move_up(Part& part, int hi, int edge, int keep_last) {
-    constexpr int ROWS = MOVE_THREADS / Part::LANES;
-    for (int i0 = 0; i0 < keep_last; i0 += ROWS * Part::BATCH) {
-        bool loaded[Part::BATCH];
+struct MoveUp {
+    static constexpr int ROWS = MOVE_THREADS / Part::LANES, BATCH = ROWS * Part::BATCH;
+    bool loaded[Part::BATCH];
+    __device__ __forceinline__ void load(Part& part, int i0, int hi, int keep_last) {
         const int mine = i0 + (int)threadIdx.x / Part::LANES;
 #pragma unroll
         for (int b = 0; b < Part::BATCH; ++b) loaded[b] = mine + b * ROWS < keep_last && part.load(b, hi + mine + b * ROWS);
-        __syncthreads();  // read by all (and what lay from the edge on has filled its holes) before any is written; the next batch's sources lie beyond this one's targets
+    }
+    __device__ __forceinline__ void store(Part& part, int i0, int edge) const {
+        const int mine = i0 + (int)threadIdx.x / Part::LANES;
 #pragma unroll
         for (int b = 0; b < Part::BATCH; ++b)
             if (loaded[b]) part.store(b, edge + mine + b * ROWS);
     }
-}
+};
 
 // A workgroup's share of a part: the first of n_shares has what may be overwritten (all moves, if it is the only one), the others the rest.
 template <typename Part>
@@ -294,8 +344,16 @@ __device__ __forceinline__ void move_part(Part part, int share, int n_shares, co
         fill(part, from, to, moves.x + (share - 1) * each, min(moves.y, moves.x + share * each));
         return;
     }
+    // the last places, from hi on, move up to the edge, a batch at a time; the first is read before the holes are filled: nothing is written from hi on
+    Part up = part;
+    MoveUp<Part> batch;
+    batch.load(up, 0, hi, keep_last);
     fill(part, from, to, 0, n_shares == 1 ? moves.y : moves.x);
-    move_up(part, hi, edge, keep_last);
+    for (int i0 = 0; i0 < keep_last; i0 += MoveUp<Part>::BATCH) {
+        if (i0 > 0) batch.load(up, i0, hi, keep_last);
+        __syncthreads();  // read by all (and what lay from the edge on has filled its holes) before any is written; the next batch's sources lie beyond this one's targets
+        batch.store(up, i0, edge);
+    }
 }
 
 // grid (sequences x heads, slices of keys and values and one for the sums, shares)
@@ -305,14 +363,20 @@ __global__ __launch_bounds__(MOVE_THREADS) void evict_move_kernel(
     const int* __restrict__ block_table, int table_width, int n_pages, int places, int max_kv, int n_kv, int head_dim, int value_dim,
     int page_size, int page_log2, int budget, int keep_last, int key_slices, int value_slices, int max_moves, const int* __restrict__ from,
     const int* __restrict__ to, const int2* __restrict__ n_moves) {
+    __shared__ int table_s[TABLE_HELD];
     const int hk = blockIdx.x % n_kv, seq = blockIdx.x / n_kv, share = blockIdx.z, n_shares = gridDim.z;
     const size_t unit = blockIdx.x;
     const int2 moves = n_moves[unit];
+    const int* const table = block_table + (size_t)seq * table_width;
+#pragma unroll
+    for (int i = 0; i < TABLE_HELD; i += MOVE_THREADS)
+        if (i + (int)threadIdx.x < table_width) table_s[i + threadIdx.x] = table[i + threadIdx.x];
+    __syncthreads();
     const int length = min(kv_len[seq], min(max_kv, places)), hi = length - keep_last, edge = budget - keep_last;
     if (moves.y < 0) return;
     from += unit * max_moves;
     to += unit * max_moves;
-    const Place at{block_table + (size_t)seq * table_width, table_width, n_pages, n_kv, hk, page_size, page_log2};
+    const Place at{table, table_s, table_width, n_pages, n_kv, hk, page_size, page_log2};
     int slice = blockIdx.y;
     if (slice < key_slices) {
         constexpr int PER = sizeof(P) / sizeof(T);
@@ -363,7 +427,7 @@ SIA_EXPORT int sia_evict(void* k_pages, void* v_pages, float* weights, const int
         if (page_size == 1 << b) page_log2 = b;
     // the widest piece that divides a key's row
     const int size = dtype == SIA_F32 ? 4 : 2, bytes = head_dim * size, piece = bytes % 16 == 0 && (uintptr_t)k_pages % 16 == 0 ? 16 : size;
-    const int lanes = min(64 / piece, 16), key_slices = (bytes / piece + lanes - 1) / lanes, value_slices = (value_dim + 7) / 8, slices = key_slices + value_slices + 1;
+    const int lanes = 4, key_slices = (bytes / piece + lanes - 1) / lanes, value_slices = (value_dim + 15) / 16, slices = key_slices + value_slices + 1;
     if (slices > 65535) return SIA_BAD_ARGUMENT;
     // further workgroups for the movers from beyond the new length, where those that there are leave the chip idle and there may be enough of them
     const ll far = max(0, min(budget - keep_last, max_kv - keep_last - budget)), there = units * slices;
@@ -373,10 +437,10 @@ SIA_EXPORT int sia_evict(void* k_pages, void* v_pages, float* weights, const int
                        (T*)v_pages, weights, slots, kv_len, block_table, table_width, n_pages, places, max_kv, n_kv, head_dim,           \
                        value_dim, page_size, page_log2, budget, keep_last, key_slices, value_slices, max_moves, from, to, n_moves)
     if (dtype == SIA_F32) {
-        if (piece == 16) LAUNCH(float, uint4);
+        if (piece == 16) LAUNCH(float, piece16);
         else LAUNCH(float, float);
     } else {
-        if (piece == 16) LAUNCH(bf16_t, uint4);
+        if (piece == 16) LAUNCH(bf16_t, piece16);
         else LAUNCH(bf16_t, bf16_t);
     }
 #undef LAUNCH
