@@ -388,7 +388,8 @@ __device__ __forceinline__ void compute_from_lds(const bf16_t* __restrict__ k_ld
 // every KSPLIT-th tile of keys: ROWS = PF_NQ * 16 * PF_WAVES / KSPLIT tokens per workgroup.  KTILES tiles of keys
 // are staged per step (and barrier); with KSPLIT = 1 every wave takes them one after the other, which at 8 waves
 // of 16 tokens is 7 % faster with two tiles than with one (fewer barriers a key) and changes no bit.
-template <int PF_NQ, int PF_WAVES, int KSPLIT, int KTILES>
+// STATS: leaves every row's m + log2(l) in row_stats (float [token][query head]).
+template <int PF_NQ, int PF_WAVES, int KSPLIT, int KTILES, bool STATS>
 __global__ __launch_bounds__(PF_WAVES* SIA_WAVE) void attn_prefill_kernel(
     const bf16_t* __restrict__ q, int q_row_stride, const bf16_t* __restrict__ kp, const bf16_t* __restrict__ vp,
     const int* __restrict__ block_table, int table_width, const int* __restrict__ cu_q,
@@ -606,7 +607,7 @@ __global__ __launch_bounds__(PF_WAVES* SIA_WAVE) void attn_prefill_kernel(
         const int row = row0 + n * 16 + r;
         if (row >= q_len) continue;
         const float total = sm.l[n] + sink_term(sinks, head, sm.m[n]), inv = 1.f / total;
-        if (row_stats && g == 0) row_stats[(size_t)(q_begin + row) * n_heads + head] = sm.m[n] + log2f(total);
+        if (STATS && g == 0) row_stats[(size_t)(q_begin + row) * n_heads + head] = sm.m[n] + log2f(total);
         bf16_t* dst = out + ((size_t)(q_begin + row) * n_heads + head) * HD;
 #pragma unroll
         for (int db = 0; db < DBLOCKS; ++db) {
@@ -796,27 +797,42 @@ SIA_EXPORT int sia_attn_prefill_rows() { return PF_ROWS; }
 SIA_EXPORT int sia_attn_prefill_rows_split() { return (HD <= 128 && PF_USE_LDS) ? PF_ROWS_SPLIT : 0; }
 SIA_EXPORT int sia_attn_prefill_rows_long() { return (HD <= 128 && PF_USE_LDS) ? PF_ROWS_LONG : 0; }
 
-template <int NQ, int WAVES, int KSPLIT, int KTILES = KSPLIT>
-static int launch_prefill(int tiles, const void* q, int q_row_stride, const void* k_pages, const void* v_pages,
-                          const int* block_table, int table_width, const int* cu_q, const int* kv_len, void* out,
-                          int seq_begin, int seq_end, int n_heads, int n_kv, int ps_log2, float scale, int window,
-                          int chunk, const float* sinks, const Forms& forms, float* row_stats, hipStream_t stream) {
+template <int NQ, int WAVES, int KSPLIT, int KTILES, bool STATS>
+static int launch_shape(int tiles, const void* q, int q_row_stride, const void* k_pages, const void* v_pages,
+                        const int* block_table, int table_width, const int* cu_q, const int* kv_len, void* out,
+                        int seq_begin, int seq_end, int n_heads, int n_kv, int ps_log2, float scale, int window,
+                        int chunk, const float* sinks, const Forms& forms, float* row_stats, hipStream_t stream) {
     constexpr int TILE_ELEMS = TILE * K_STRIDE + HD * V_STRIDE;
     size_t lds_bytes = PF_USE_LDS ? (size_t)2 * KTILES * TILE_ELEMS * sizeof(bf16_t) : 0;
     if (KSPLIT == 2) {
         const size_t merge = (size_t)(WAVES / 2) * SIA_WAVE * NQ * (DBLOCKS * 4 + 2) * sizeof(float);
         if (merge > lds_bytes) lds_bytes = merge;
     }
-    const void* fn = reinterpret_cast<const void*>(&attn_prefill_kernel<NQ, WAVES, KSPLIT, KTILES>);
+    const void* fn = reinterpret_cast<const void*>(&attn_prefill_kernel<NQ, WAVES, KSPLIT, KTILES, STATS>);
     if (lds_bytes > 48 * 1024) {  // beyond the default limit of dynamic LDS
         const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes);
         if (e != hipSuccess) return (int)e;
     }
-    hipLaunchKernelGGL((attn_prefill_kernel<NQ, WAVES, KSPLIT, KTILES>), dim3(tiles, n_heads), dim3(WAVES * SIA_WAVE),
+    hipLaunchKernelGGL((attn_prefill_kernel<NQ, WAVES, KSPLIT, KTILES, STATS>), dim3(tiles, n_heads), dim3(WAVES * SIA_WAVE),
                        lds_bytes, stream, (const bf16_t*)q, q_row_stride, (const bf16_t*)k_pages,
                        (const bf16_t*)v_pages, block_table, table_width, cu_q, kv_len, (bf16_t*)out, n_heads, n_kv,
                        ps_log2, scale, window, chunk, sinks, seq_begin, seq_end, forms, row_stats);
     return SIA_LAUNCH_CHECK();
+}
+
+template <int NQ, int WAVES, int KSPLIT, int KTILES = KSPLIT>
+static int launch_prefill(int tiles, const void* q, int q_row_stride, const void* k_pages, const void* v_pages,
+                          const int* block_table, int table_width, const int* cu_q, const int* kv_len, void* out,
+                          int seq_begin, int seq_end, int n_heads, int n_kv, int ps_log2, float scale, int window,
+                          int chunk, const float* sinks, const Forms& forms, float* row_stats, hipStream_t stream) {
+    if constexpr (!FORMS)      // the statistics go without the forms
+        if (row_stats)
+            return launch_shape<NQ, WAVES, KSPLIT, KTILES, true>(tiles, q, q_row_stride, k_pages, v_pages, block_table, table_width, cu_q, kv_len, out,
+                                                                 seq_begin, seq_end, n_heads, n_kv, ps_log2, scale, window, chunk, sinks, forms,
+                                                                 row_stats, stream);
+    return launch_shape<NQ, WAVES, KSPLIT, KTILES, false>(tiles, q, q_row_stride, k_pages, v_pages, block_table, table_width, cu_q, kv_len, out,
+                                                          seq_begin, seq_end, n_heads, n_kv, ps_log2, scale, window, chunk, sinks, forms,
+                                                          row_stats, stream);
 }
 
 // Which of the four workgroup shapes a launch takes.  n_tiles, n_tiles_split, n_tiles_long: its row tiles at 128, 64
@@ -922,7 +938,7 @@ SIA_EXPORT int sia_attn_prefill_stats(const void* q, int q_row_stride, const voi
                                       void* out, int seq_begin, int seq_end, int n_tiles, int n_tiles_split,
                                       int n_tiles_long, int q_bound, int kv_bound, int n_heads, int n_kv, int page_size,
                                       float scale, const float* sinks, float* row_stats, hipStream_t stream) {
-    if (!row_stats) return SIA_BAD_ARGUMENT;
+    if (FORMS || !row_stats) return SIA_BAD_ARGUMENT;
     return prefill(q, q_row_stride, k_pages, v_pages, block_table, table_width, cu_q, kv_len, out, seq_begin, seq_end, n_tiles,
                    n_tiles_split, n_tiles_long, q_bound, kv_bound, n_heads, n_kv, page_size, scale, 0, 0, sinks, 0.f, 0, row_stats,
                    stream);
