@@ -107,6 +107,15 @@ class PagedGroup:
             table.extend(self.pool.take_many(req, more))
             self._touch(req)
 
+    def shrink(self, req: int, tokens: int) -> None:
+        """Gives back the pages behind place ``tokens - 1``; the request may take as many again."""
+        table, keep = self.tables[req], pages_for(tokens, self.page_size)
+        if len(table) > keep:
+            for page in table[keep:]:
+                self.pool.drop(req, page, restore_promise=True)
+            del table[keep:]
+            self._touch(req)
+
     def _touch(self, req: int) -> None:
         self._version += 1
         self.versions[req] = self._version
@@ -221,6 +230,25 @@ class CacheManager:
         if not 0 <= tokens <= self.lengths[req]:
             raise ValueError(f"request {req} holds {self.lengths[req]} tokens and cannot go back {tokens}")
         self.lengths[req] -= tokens
+
+    def owns_pages(self, req: int) -> bool:
+        """Whether every page of the request is its own (and none that of a shared or kept prefix): what an eviction, which
+        moves rows within them, asks for."""
+        return all(g.pool.holders(p) == 1 for g in self.groups for p in g.pool.pages(req))
+
+    def shrink(self, req: int, tokens: int) -> None:
+        """After an eviction (``HipKernels.evict_cache`` for every layer) that left the request ``tokens`` places: its next token
+        goes to place ``tokens``, and the pages behind the last place go back to the pool, promised to the request.  From
+        then on a token's place is not its position any more, so there are neither windows nor blocks of positions."""
+        if not 0 < tokens <= self.lengths[req]:
+            raise ValueError(f"request {req} holds {self.lengths[req]} tokens and cannot keep {tokens}")
+        if any(g.need.span is not None for g in self.groups):
+            raise ValueError("a cache with a window or blocks knows its keys by their positions")
+        if not self.owns_pages(req):
+            raise ValueError(f"request {req} shares pages")
+        for g in self.groups:
+            g.shrink(req, tokens)
+        self.lengths[req] = tokens
 
     def release(self, req: int) -> None:
         for g in self.groups:
