@@ -7,8 +7,8 @@
 // the values is needed, only the scores again.  A place that the step itself has written begins at zero, whatever lay there.
 // All sums are float, each made by one thread in a fixed order.
 //
-// Float heads of up to 128 go by the float matrix cores (weigh_f32_kernel), with keys as rows and queries as columns, single tokens and
-// runs alike; bfloat16 heads of 16 to 256 by attention_weighed_mfma.hip.
+// Heads of up to 256 in fours go by the float matrix cores (weigh_float_kernel), with keys as rows and queries as columns, single tokens and
+// runs alike; bfloat16 heads that the attention kernels take on the bfloat16 matrix cores by attention_weighed_mfma.hip.
 // The plain kernel: a wave for 64 consecutive places of one (sequence, key/value head), a lane a key; the queries come one after
 // the other through LDS.  It takes every head size, page size and type.
 #include "f32_lanes.h"
@@ -74,20 +74,29 @@ SIA_EXPORT int sia_weigh_plain(const void* q, int q_row_stride, const void* k_pa
 }
 
 // ---------------------------------------------------------------------------------------------------
-// float heads of up to 128 on the float matrix cores (v_mfma_f32_16x16x4_f32)
+// heads of up to 256 on the float matrix cores (v_mfma_f32_16x16x4_f32)
 // ---------------------------------------------------------------------------------------------------
 // A dot product's elements come in the attention kernels' order, so that a score has the bits that went into its row's statistic: what is
 // left of a weight's error is that of two exponentials and a sum.  (In the order in which a lane loads them, without the exchange between
 // lanes, errors of 8e-7 of the sums where 2e-7 are now.)
-constexpr int F32_WAVES = 4, F32_BLOCKS = 2, F32_WAVE_KEYS = 16 * F32_BLOCKS, F32_KEYS = F32_WAVES * F32_WAVE_KEYS;
+constexpr int F32_WAVES = 4;
+// Blocks of 16 keys of a wave, and keys of a workgroup: what the registers hold.
+constexpr int f32_blocks(int dp) { return dp <= 128 ? 2 : 1; }
+constexpr int f32_keys(int dp) { return F32_WAVES * 16 * f32_blocks(dp); }
 
-// DP: 32, 64 or 128, the head sizes' upper bound.  grid and parts as weigh_runs_kernel's.
-template <int DP>
-__global__ __launch_bounds__(F32_WAVES* SIA_WAVE) void weigh_f32_kernel(
-    const float* __restrict__ q, int q_row_stride, const float* __restrict__ k_pages, const int* __restrict__ block_table, int table_width,
+__device__ __forceinline__ f32x4 load4(const float* p) { return *(const f32x4*)p; }
+__device__ __forceinline__ f32x4 load4(const bf16_t* p) {
+    const uint2 u = *(const uint2*)p;
+    return f32x4{__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u)};
+}
+
+// DP: 32, 64, 128 or 256, the head sizes' upper bound.  grid and parts as weigh_runs_kernel's.
+template <typename T, int DP>
+__global__ __launch_bounds__(F32_WAVES* SIA_WAVE) void weigh_float_kernel(
+    const T* __restrict__ q, int q_row_stride, const T* __restrict__ k_pages, const int* __restrict__ block_table, int table_width,
     const int* __restrict__ cu_q, const int* __restrict__ kv_len, const float* __restrict__ row_stats, int n_heads, int n_kv, int head_dim,
     int page_size, int n_pages, float scale, int chunk_rows, int most_keys, float* __restrict__ parts, const Weighed w) {
-    constexpr int PIECES = DP / 16;
+    constexpr int PIECES = DP / 16, F32_BLOCKS = f32_blocks(DP), F32_WAVE_KEYS = 16 * F32_BLOCKS, F32_KEYS = f32_keys(DP);
     const int hk = blockIdx.x, group = n_heads / n_kv;
     Work run;
     if (!find_work<F32_KEYS>(run, blockIdx.y, blockIdx.z, cu_q, kv_len, group, chunk_rows, most_keys)) return;
@@ -95,11 +104,11 @@ __global__ __launch_bounds__(F32_WAVES* SIA_WAVE) void weigh_f32_kernel(
     const int k0 = run.key0 + wave * F32_WAVE_KEYS;
     if (k0 >= run.length) return;
     const int* table = block_table + (size_t)run.seq * table_width;
-    auto load_row = [&](f32x4 (&x)[PIECES], const float* row) {
+    auto load_row = [&](f32x4 (&x)[PIECES], const T* row) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             const int d = 16 * i + 4 * g;
-            x[i] = *(const f32x4*)(row + (d < head_dim ? d : 0));
+            x[i] = load4(row + (d < head_dim ? d : 0));
             if (d >= head_dim) x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
             across_groups(x[i]);
         }
@@ -167,45 +176,56 @@ __global__ __launch_bounds__(F32_WAVES* SIA_WAVE) void weigh_f32_kernel(
     leave_sums(sum, k0, run, parts ? parts + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * n_kv + hk) * F32_KEYS : nullptr, w, n_kv, hk);
 }
 
-// Whether weigh_f32_kernel takes such heads (and rows of q and keys in sixteens of bytes).
-SIA_EXPORT int sia_weigh_f32_takes(int head_dim) { return head_dim > 0 && head_dim <= 128 && head_dim % 4 == 0; }
+// Whether weigh_float_kernel takes such heads (and rows of q and keys in fours of elements).
+SIA_EXPORT int sia_weigh_float_takes(int head_dim) { return head_dim > 0 && head_dim <= 256 && head_dim % 4 == 0; }
 
 // How the sequences of a launch are cut: three workgroups are on a compute unit at a time.
-static Cut cut_f32(int total_tokens, int q_bound, int n_seqs, int max_kv, int n_heads, int n_kv) {
-    return cut_runs(total_tokens, q_bound, n_seqs, max_kv, n_heads / n_kv, n_kv, F32_KEYS, 64, 768);
+static Cut cut_float(int total_tokens, int q_bound, int n_seqs, int max_kv, int n_heads, int n_kv, int head_dim) {
+    return cut_runs(total_tokens, q_bound, n_seqs, max_kv, n_heads / n_kv, n_kv, f32_keys(head_dim), 64, 768);
 }
 
-// Floats of sia_weigh_f32's workspace (0: none).
-SIA_EXPORT long long sia_weigh_f32_workspace(int total_tokens, int q_bound, int n_seqs, int max_kv, int n_heads, int n_kv) {
+// Floats of sia_weigh_float's workspace (0: none).
+SIA_EXPORT long long sia_weigh_float_workspace(int total_tokens, int q_bound, int n_seqs, int max_kv, int n_heads, int n_kv, int head_dim) {
     if (total_tokens <= 0 || q_bound <= 0 || n_seqs <= 0 || max_kv <= 0 || n_kv <= 0 || n_heads % n_kv) return 0;
-    return cut_f32(total_tokens, q_bound, n_seqs, max_kv, n_heads, n_kv).floats;
+    return cut_float(total_tokens, q_bound, n_seqs, max_kv, n_heads, n_kv, head_dim).floats;
 }
 
 // As sia_weigh_plain, single tokens and runs alike; total_tokens in all, no sequence with more than q_bound tokens.
-SIA_EXPORT int sia_weigh_f32(const float* q, int q_row_stride, const float* k_pages, const int* block_table, int table_width, const int* cu_q,
-                             const int* kv_len, const int* slots, const float* row_stats, float* weights, int n_slots, int places, int n_seqs,
-                             int max_kv, int n_heads, int n_kv, int head_dim, int page_size, int n_pages, float scale, int total_tokens, int q_bound,
-                             float* ws, hipStream_t stream) {
+SIA_EXPORT int sia_weigh_float(const void* q, int q_row_stride, const void* k_pages, const int* block_table, int table_width, const int* cu_q,
+                               const int* kv_len, const int* slots, const float* row_stats, float* weights, int n_slots, int places, int n_seqs,
+                               int max_kv, int n_heads, int n_kv, int head_dim, int page_size, int n_pages, float scale, int total_tokens, int q_bound,
+                               float* ws, int dtype, hipStream_t stream) {
     if (n_seqs <= 0 || max_kv <= 0 || total_tokens <= 0 || q_bound <= 0) return 0;
-    if (!sia_weigh_f32_takes(head_dim) || q_row_stride % 4 || ((uintptr_t)q | (uintptr_t)k_pages) % 16 || n_kv <= 0 || n_heads % n_kv || page_size <= 0 ||
-        n_seqs > 65535 || places < max_kv || table_width <= 0 || n_pages <= 0 || n_slots <= 0 || (long long)q_bound * (n_heads / n_kv) > 0x7fffff00)
+    if ((dtype != SIA_F32 && dtype != SIA_BF16) || !sia_weigh_float_takes(head_dim) || q_row_stride % 4 || ((uintptr_t)q | (uintptr_t)k_pages) % (dtype == SIA_F32 ? 16 : 8) ||
+        n_kv <= 0 || n_heads % n_kv || page_size <= 0 || n_seqs > 65535 || places < max_kv || table_width <= 0 || n_pages <= 0 || n_slots <= 0 ||
+        (long long)q_bound * (n_heads / n_kv) > 0x7fffff00)
         return SIA_BAD_ARGUMENT;
-    const Cut cut = cut_f32(total_tokens, q_bound, n_seqs, max_kv, n_heads, n_kv);
-    const int blocks = (max_kv + F32_KEYS - 1) / F32_KEYS;
+    const Cut cut = cut_float(total_tokens, q_bound, n_seqs, max_kv, n_heads, n_kv, head_dim);
+    const int blocks = (max_kv + f32_keys(head_dim) - 1) / f32_keys(head_dim);
     if (cut.most_work > 65535 || blocks > 65535 || (cut.floats && !ws)) return SIA_BAD_ARGUMENT;
     const Weighed w{weights, slots, nullptr, n_slots, places, 0};
     const int most_keys = (int)min((long long)max_kv, (long long)table_width * page_size);
     float* parts = cut.floats ? ws : nullptr;
-#define LAUNCH(DP)                                                                                                                          \
-    hipLaunchKernelGGL(weigh_f32_kernel<DP>, dim3(n_kv, cut.most_work, n_seqs), dim3(F32_WAVES * SIA_WAVE), 0, stream, q, q_row_stride,       \
-                       k_pages, block_table, table_width, cu_q, kv_len, row_stats, n_heads, n_kv, head_dim, page_size, n_pages, scale,       \
-                       cut.chunk_rows, most_keys, parts, w)
-    if (head_dim <= 32) LAUNCH(32);
-    else if (head_dim <= 64) LAUNCH(64);
-    else LAUNCH(128);
+#define LAUNCH(T, DP)                                                                                                                       \
+    do {                                                                                                                                    \
+        hipLaunchKernelGGL((weigh_float_kernel<T, DP>), dim3(n_kv, cut.most_work, n_seqs), dim3(F32_WAVES * SIA_WAVE), 0, stream,           \
+                           (const T*)q, q_row_stride, (const T*)k_pages, block_table, table_width, cu_q, kv_len, row_stats, n_heads, n_kv, \
+                           head_dim, page_size, n_pages, scale, cut.chunk_rows, most_keys, parts, w);                                      \
+        if (parts)                                                                                                                          \
+            hipLaunchKernelGGL(weigh_add_kernel<f32_keys(DP)>, dim3(n_kv, blocks, n_seqs), dim3(f32_keys(DP)), 0, stream, parts, cu_q,       \
+                               kv_len, n_heads, n_kv, 0, cut.chunk_rows, most_keys, cut.most_work, w);                                     \
+    } while (0)
+#define OF_TYPE(T)                          \
+    if (head_dim <= 32) LAUNCH(T, 32);      \
+    else if (head_dim <= 64) LAUNCH(T, 64); \
+    else if (head_dim <= 128) LAUNCH(T, 128); \
+    else LAUNCH(T, 256)
+    if (dtype == SIA_F32) {
+        OF_TYPE(float);
+    } else {
+        OF_TYPE(bf16_t);
+    }
+#undef OF_TYPE
 #undef LAUNCH
-    if (parts)
-        hipLaunchKernelGGL(weigh_add_kernel<F32_KEYS>, dim3(n_kv, blocks, n_seqs), dim3(F32_KEYS), 0, stream, parts, cu_q, kv_len, n_heads, n_kv, 0,
-                           cut.chunk_rows, most_keys, cut.most_work, w);
     return SIA_LAUNCH_CHECK();
 }

@@ -115,10 +115,10 @@ _SIGNATURES = {
                         _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_ptr],
     "sia_attention_f32_stats": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
                                 _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_ptr, _c_ptr],
-    "sia_weigh_f32_takes": [_c_int],
-    "sia_weigh_f32_workspace": [_c_int] * 6,
-    "sia_weigh_f32": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
-                      _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
+    "sia_weigh_float_takes": [_c_int],
+    "sia_weigh_float_workspace": [_c_int] * 7,
+    "sia_weigh_float": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
+                        _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_int, _c_ptr],
     "sia_rope_axes_max": [],
     "sia_rope_axes_kv_write": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int,
                                _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr],
@@ -355,7 +355,7 @@ class HipKernels:
         self.core.sia_delta_rule_workspace.restype = ctypes.c_longlong
         self.core.sia_linear_unit_workspace.restype = ctypes.c_longlong
         self.core.sia_bonus_recurrence_workspace.restype = ctypes.c_longlong
-        self.core.sia_evict_workspace.restype = self.core.sia_weigh_f32_workspace.restype = ctypes.c_longlong
+        self.core.sia_evict_workspace.restype = self.core.sia_weigh_float_workspace.restype = ctypes.c_longlong
         self.tiled_experts = True        # many slots in bfloat16: experts' products on the matrix cores, slots sorted by expert
         self._attn_libs = {}
         # the short way to the current stream's handle, where this torch has it (a few microseconds less a launch)
@@ -2112,24 +2112,21 @@ class HipKernels:
                 _ptr(qkv), width, _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(table), table.shape[1], _ptr(ctx.seq_of_token),
                 _ptr(ctx.positions), _ptr(out), n, ctx.n_decode_seqs, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim, value_dim, page,
                 float(scale), _ptr(sinks), _ptr(stats), stream), "attention_f32_stats")
-            if self.core.sia_weigh_f32_takes(head_dim) and width % 4 == 0 and _in_pieces(qkv, cache.k_pages):
-                q_bound = max(ctx.q_lens)
-                floats = self.core.sia_weigh_f32_workspace(n, q_bound, ctx.n_seqs, max_kv, n_heads, n_kv_heads)
-                ws = weights.new_empty((floats,)) if floats else None
-                self._check(self.core.sia_weigh_f32(
-                    _ptr(qkv), width, _ptr(cache.k_pages), _ptr(table), table.shape[1], _ptr(ctx.cu_q), _ptr(ctx.kv_len),
-                    _ptr(ctx.state_slots), _ptr(stats), _ptr(weights), *places, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim, page,
-                    pages, float(scale), n, q_bound, _ptr(ws), stream), "weigh_f32")
-                return out
         else:
             self._check(self.core.sia_attention_generic_stats(
                 _ptr(qkv), width, _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(table), table.shape[1], _ptr(ctx.seq_of_token),
                 _ptr(ctx.positions), _ptr(out), n, n_heads, n_kv_heads, head_dim, value_dim, page, float(scale), _ptr(sinks), _ptr(stats),
                 _DT[qkv.dtype], stream), "attention_generic_stats")
-        self._check(self.core.sia_weigh_plain(
-            _ptr(qkv), width, _ptr(cache.k_pages), _ptr(table), table.shape[1], _ptr(ctx.cu_q), _ptr(ctx.kv_len),
-            _ptr(ctx.state_slots), _ptr(stats), _ptr(weights), *places, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim, page, pages,
-            float(scale), _DT[qkv.dtype], stream), "weigh_plain")
+        weigh = (_ptr(qkv), width, _ptr(cache.k_pages), _ptr(table), table.shape[1], _ptr(ctx.cu_q), _ptr(ctx.kv_len),
+                 _ptr(ctx.state_slots), _ptr(stats), _ptr(weights), *places, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim, page,
+                 pages, float(scale))
+        if self.core.sia_weigh_float_takes(head_dim) and width % 4 == 0 and _in_pieces(qkv, cache.k_pages):
+            q_bound = max(ctx.q_lens)
+            floats = self.core.sia_weigh_float_workspace(n, q_bound, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim)
+            ws = weights.new_empty((floats,)) if floats else None
+            self._check(self.core.sia_weigh_float(*weigh, n, q_bound, _ptr(ws), _DT[qkv.dtype], stream), "weigh_float")
+        else:
+            self._check(self.core.sia_weigh_plain(*weigh, _DT[qkv.dtype], stream), "weigh_plain")
         return out
 
     def _weighed_mfma(self, qkv, out, n_heads, n_kv, head_dim, scale, ctx, cache, sinks, weights, max_kv):

@@ -33,7 +33,7 @@ class Ctx:
     def __init__(self, q_lens, kv_lens, slots=None, kv_bound=0):
         pos, sot, cu = [], [], [0]
         for s, (q, kv) in enumerate(zip(q_lens, kv_lens)):
-            pos += list(range(kv - q, kv))
+            pos += list(range(kv - q, kv))      # (a sequence without places: place -1)
             sot += [s] * q
             cu.append(cu[-1] + q)
         i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
@@ -227,7 +227,8 @@ def check_weighed(hip, ctx, cache, qkv, heads, scale, sinks=None, poison=True):
     cu, lens, slots = ctx.cu_q.tolist(), ctx.kv_len.tolist(), ctx.state_slots.tolist()
     if poison:      # whatever lies where the step writes is no part of the sums
         for s, length in enumerate(lens):
-            cache.weights[slots[s], :, length - (cu[s + 1] - cu[s]):length] = math.nan
+            if length > 0:
+                cache.weights[slots[s], :, length - (cu[s + 1] - cu[s]):length] = math.nan
     before = cache.weights.clone()
     out = hip.weighed_attention(qkv, heads, kv, dim, scale, ctx, cache, value_dim=vdim, sinks=sinks)
     assert out.shape == (ctx.n_tokens, heads * vdim) and out.dtype == dtype
@@ -287,6 +288,9 @@ ATTENTIONS = [
     ([1, 1, 300], [150, 260, 300], 32, 8, 64, 16),
     ([5, 1], [5, 9], 2, 1, 20, 12),                                # odd heads, pages of no power of two
     ([1, 30], [50, 41], 3, 3, 36, 4),
+    ([70, 1, 9], [300, 5, 9], 6, 2, 22, 12),                       # heads that are not in fours
+    ([1, 45], [90, 200], 4, 2, 200, 16),
+    ([1] * 3, [0, 3, 0], 4, 2, 64, 16),                            # sequences without places
     ([1], [130], 4, 4, 256, 16),
 ]
 
@@ -303,7 +307,7 @@ def test_weighed_attention(hip, dtype, q_lens, kv_lens, heads, kv, dim, page):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("q_lens,kv_lens,heads,kv,dim,vdim,page", [([1, 45], [200, 60], 6, 2, 64, 32, 16), ([1, 1], [40, 600], 4, 4, 48, 96, 8),
-                                                                  ([9], [30], 2, 1, 640, 512, 16)])
+                                                                  ([9], [30], 2, 1, 640, 512, 16), ([1, 400], [900, 450], 8, 2, 128, 64, 16)])
 def test_weighed_attention_with_values_of_another_width(hip, dtype, q_lens, kv_lens, heads, kv, dim, vdim, page):
     ctx, cache = Ctx(q_lens, kv_lens), Cache(kv_lens, kv, page, dim, dtype, value_dim=vdim)
     check_weighed(hip, ctx, cache, rnd(ctx.n_tokens, heads * dim, dtype=dtype, seed=8), heads, dim ** -0.5)
