@@ -51,25 +51,12 @@ __global__ __launch_bounds__(SIA_WAVE) void weigh_plain_kernel(
     if (j < length) row[j] = (j < start ? row[j] : 0.f) + total;
 }
 
-// q: rows of the step's tokens, n_heads * head_dim columns first; cu_q, kv_len, slots: per sequence; row_stats [tokens][n_heads];
-// weights [n_slots][n_kv][places]; max_kv: no sequence holds more (what the grid is sized by).
-SIA_EXPORT int sia_weigh_plain(const void* q, int q_row_stride, const void* k_pages, const int* block_table, int table_width,
-                               const int* cu_q, const int* kv_len, const int* slots, const float* row_stats, float* weights,
-                               int n_slots, int places, int n_seqs, int max_kv, int n_heads, int n_kv, int head_dim, int page_size,
-                               int n_pages, float scale, int dtype, hipStream_t stream) {
-    if (n_seqs <= 0 || max_kv <= 0) return 0;
-    if (head_dim <= 0 || head_dim > WEIGH_MAX_HEAD_DIM || n_kv <= 0 || n_heads % n_kv || page_size <= 0 || n_kv > 65535 || n_seqs > 65535 ||
-        places <= 0 || table_width <= 0 || n_pages <= 0)
-        return SIA_BAD_ARGUMENT;
-    const Weighed w{weights, slots, nullptr, n_slots, places, 0};
-    const dim3 grid((max_kv + SIA_WAVE - 1) / SIA_WAVE, n_kv, n_seqs);
-#define LAUNCH(T)                                                                                                                   \
-    hipLaunchKernelGGL(weigh_plain_kernel<T>, grid, dim3(SIA_WAVE), 0, stream, (const T*)q, q_row_stride, (const T*)k_pages,        \
-                       block_table, table_width, cu_q, kv_len, row_stats, n_heads, n_kv, head_dim, page_size, n_pages, scale, w)
-    if (dtype == SIA_F32) LAUNCH(float);
-    else if (dtype == SIA_BF16) LAUNCH(bf16_t);
-    else return SIA_BAD_ARGUMENT;
-#undef LAUNCH
+template <typename T>
+static int weigh_plain(const T* q, int q_row_stride, const T* k_pages, const int* block_table, int table_width, const int* cu_q, const int* kv_len,
+                       const float* row_stats, int n_seqs, int max_kv, int n_heads, int n_kv, int head_dim, int page_size, int n_pages, float scale,
+                       const Weighed& w, hipStream_t stream) {
+    hipLaunchKernelGGL(weigh_plain_kernel<T>, dim3((max_kv + SIA_WAVE - 1) / SIA_WAVE, n_kv, n_seqs), dim3(SIA_WAVE), 0, stream, q, q_row_stride,
+                       k_pages, block_table, table_width, cu_q, kv_len, row_stats, n_heads, n_kv, head_dim, page_size, n_pages, scale, w);
     return SIA_LAUNCH_CHECK();
 }
 
@@ -176,56 +163,80 @@ __global__ __launch_bounds__(F32_WAVES* SIA_WAVE) void weigh_float_kernel(
     leave_sums(sum, k0, run, parts ? parts + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * n_kv + hk) * F32_KEYS : nullptr, w, n_kv, hk);
 }
 
-// Whether weigh_float_kernel takes such heads (and rows of q and keys in fours of elements).
-SIA_EXPORT int sia_weigh_float_takes(int head_dim) { return head_dim > 0 && head_dim <= 256 && head_dim % 4 == 0; }
+// Whether weigh_float_kernel takes such heads and rows.
+static bool float_takes(const void* q, int q_row_stride, const void* k_pages, int head_dim, int dtype) {
+    return head_dim <= 256 && head_dim % 4 == 0 && q_row_stride % 4 == 0 && ((uintptr_t)q | (uintptr_t)k_pages) % (dtype == SIA_F32 ? 16 : 8) == 0;
+}
 
 // How the sequences of a launch are cut: three workgroups are on a compute unit at a time.
-static Cut cut_float(int total_tokens, int q_bound, int n_seqs, int max_kv, int n_heads, int n_kv, int head_dim) {
-    return cut_runs(total_tokens, q_bound, n_seqs, max_kv, n_heads / n_kv, n_kv, f32_keys(head_dim), 64, 768);
+static Cut cut_float(int n_tokens, int q_bound, int n_seqs, int max_kv, int n_heads, int n_kv, int head_dim) {
+    return cut_runs(n_tokens, q_bound, n_seqs, max_kv, n_heads / n_kv, n_kv, f32_keys(head_dim), 64, 768);
 }
 
-// Floats of sia_weigh_float's workspace (0: none).
-SIA_EXPORT long long sia_weigh_float_workspace(int total_tokens, int q_bound, int n_seqs, int max_kv, int n_heads, int n_kv, int head_dim) {
-    if (total_tokens <= 0 || q_bound <= 0 || n_seqs <= 0 || max_kv <= 0 || n_kv <= 0 || n_heads % n_kv) return 0;
-    return cut_float(total_tokens, q_bound, n_seqs, max_kv, n_heads, n_kv, head_dim).floats;
-}
-
-// As sia_weigh_plain, single tokens and runs alike; total_tokens in all, no sequence with more than q_bound tokens.
-SIA_EXPORT int sia_weigh_float(const void* q, int q_row_stride, const void* k_pages, const int* block_table, int table_width, const int* cu_q,
-                               const int* kv_len, const int* slots, const float* row_stats, float* weights, int n_slots, int places, int n_seqs,
-                               int max_kv, int n_heads, int n_kv, int head_dim, int page_size, int n_pages, float scale, int total_tokens, int q_bound,
-                               float* ws, int dtype, hipStream_t stream) {
-    if (n_seqs <= 0 || max_kv <= 0 || total_tokens <= 0 || q_bound <= 0) return 0;
-    if ((dtype != SIA_F32 && dtype != SIA_BF16) || !sia_weigh_float_takes(head_dim) || q_row_stride % 4 || ((uintptr_t)q | (uintptr_t)k_pages) % (dtype == SIA_F32 ? 16 : 8) ||
-        n_kv <= 0 || n_heads % n_kv || page_size <= 0 || n_seqs > 65535 || places < max_kv || table_width <= 0 || n_pages <= 0 || n_slots <= 0 ||
-        (long long)q_bound * (n_heads / n_kv) > 0x7fffff00)
-        return SIA_BAD_ARGUMENT;
-    const Cut cut = cut_float(total_tokens, q_bound, n_seqs, max_kv, n_heads, n_kv, head_dim);
-    const int blocks = (max_kv + f32_keys(head_dim) - 1) / f32_keys(head_dim);
-    if (cut.most_work > 65535 || blocks > 65535 || (cut.floats && !ws)) return SIA_BAD_ARGUMENT;
-    const Weighed w{weights, slots, nullptr, n_slots, places, 0};
-    const int most_keys = (int)min((long long)max_kv, (long long)table_width * page_size);
-    float* parts = cut.floats ? ws : nullptr;
-#define LAUNCH(T, DP)                                                                                                                       \
-    do {                                                                                                                                    \
-        hipLaunchKernelGGL((weigh_float_kernel<T, DP>), dim3(n_kv, cut.most_work, n_seqs), dim3(F32_WAVES * SIA_WAVE), 0, stream,           \
-                           (const T*)q, q_row_stride, (const T*)k_pages, block_table, table_width, cu_q, kv_len, row_stats, n_heads, n_kv, \
-                           head_dim, page_size, n_pages, scale, cut.chunk_rows, most_keys, parts, w);                                      \
-        if (parts)                                                                                                                          \
-            hipLaunchKernelGGL(weigh_add_kernel<f32_keys(DP)>, dim3(n_kv, blocks, n_seqs), dim3(f32_keys(DP)), 0, stream, parts, cu_q,       \
-                               kv_len, n_heads, n_kv, 0, cut.chunk_rows, most_keys, cut.most_work, w);                                     \
-    } while (0)
-#define OF_TYPE(T)                          \
-    if (head_dim <= 32) LAUNCH(T, 32);      \
-    else if (head_dim <= 64) LAUNCH(T, 64); \
-    else if (head_dim <= 128) LAUNCH(T, 128); \
-    else LAUNCH(T, 256)
-    if (dtype == SIA_F32) {
-        OF_TYPE(float);
-    } else {
-        OF_TYPE(bf16_t);
-    }
-#undef OF_TYPE
-#undef LAUNCH
+template <typename T, int DP>
+static int weigh_float(const T* q, int q_row_stride, const T* k_pages, const int* block_table, int table_width, const int* cu_q, const int* kv_len,
+                       const float* row_stats, float* parts, int n_seqs, int max_kv, int n_heads, int n_kv, int head_dim, int page_size, int n_pages,
+                       float scale, const Cut& cut, const Weighed& w, hipStream_t stream) {
+    const int most_keys = (int)min((long long)max_kv, (long long)table_width * page_size), blocks = (max_kv + f32_keys(DP) - 1) / f32_keys(DP);
+    if (cut.most_work > 65535 || blocks > 65535) return SIA_BAD_ARGUMENT;
+    hipLaunchKernelGGL((weigh_float_kernel<T, DP>), dim3(n_kv, cut.most_work, n_seqs), dim3(F32_WAVES * SIA_WAVE), 0, stream, q, q_row_stride, k_pages,
+                       block_table, table_width, cu_q, kv_len, row_stats, n_heads, n_kv, head_dim, page_size, n_pages, scale, cut.chunk_rows,
+                       most_keys, parts, w);
+    if (parts)
+        hipLaunchKernelGGL(weigh_add_kernel<f32_keys(DP)>, dim3(n_kv, blocks, n_seqs), dim3(f32_keys(DP)), 0, stream, parts, cu_q, kv_len, n_heads,
+                           n_kv, 0, cut.chunk_rows, most_keys, cut.most_work, w);
     return SIA_LAUNCH_CHECK();
+}
+
+// ---------------------------------------------------------------------------------------------------
+// entry points
+// ---------------------------------------------------------------------------------------------------
+extern "C" int sia_attention_f32_stats(const float*, int, const float*, const float*, const int*, int, const int*, const int*, float*, int, int, int,
+                                       int, int, int, int, int, int, float, const float*, float*, hipStream_t);
+extern "C" int sia_attention_generic_stats(const void*, int, const void*, const void*, const int*, int, const int*, const int*, void*, int, int, int,
+                                           int, int, int, float, const float*, float*, int, hipStream_t);
+
+// Floats that sia_attention_weighed's workspace holds (arguments as there).
+SIA_EXPORT long long sia_attention_weighed_workspace(int n_tokens, int q_bound, int n_seqs, int max_kv, int n_heads, int n_kv, int head_dim) {
+    if (n_tokens <= 0 || q_bound <= 0 || n_seqs <= 0 || max_kv <= 0 || n_heads <= 0 || n_kv <= 0 || n_heads % n_kv) return 0;
+    return (long long)n_tokens * n_heads + cut_float(n_tokens, q_bound, n_seqs, max_kv, n_heads, n_kv, head_dim).floats;
+}
+
+// The arguments of the attention kernels without window, blocks and forms; q: rows of the step's tokens; n_single: that many sequences, the first
+// ones, bring one token each; none of them more than q_bound tokens, n_tokens in all, over at most max_kv places; weights [n_slots][n_kv][places], a
+// sequence's row at slots[s].
+SIA_EXPORT int sia_attention_weighed(const void* q, int q_row_stride, const void* k_pages, const void* v_pages, const int* block_table, int table_width,
+                                     const int* seq_of_token, const int* positions, const int* cu_q, const int* kv_len, void* out, float* ws,
+                                     int n_tokens, int n_single, int n_seqs, int q_bound, int max_kv, int n_heads, int n_kv, int head_dim,
+                                     int value_dim, int page_size, int n_pages, float scale, const float* sinks, float* weights, const int* slots,
+                                     int n_slots, int places, int dtype, hipStream_t stream) {
+    if (n_tokens <= 0 || n_seqs <= 0) return 0;
+    if ((dtype != SIA_F32 && dtype != SIA_BF16) || head_dim <= 0 || head_dim > WEIGH_MAX_HEAD_DIM || value_dim <= 0 || n_heads <= 0 || n_kv <= 0 || n_heads % n_kv ||
+        n_heads > 65535 || n_seqs > 65535 || page_size <= 0 || table_width <= 0 || n_pages <= 0 || q_bound <= 0 || max_kv <= 0 || places < max_kv ||
+        n_slots <= 0 || !ws || !weights || (long long)q_bound * (n_heads / n_kv) > 0x7fffff00)
+        return SIA_BAD_ARGUMENT;
+    float* stats = ws;
+    int rc = dtype == SIA_F32 ? sia_attention_f32_stats((const float*)q, q_row_stride, (const float*)k_pages, (const float*)v_pages, block_table, table_width,
+                                                        seq_of_token, positions, (float*)out, n_tokens, n_single, n_seqs, max_kv, n_heads, n_kv,
+                                                        head_dim, value_dim, page_size, scale, sinks, stats, stream)
+                              : sia_attention_generic_stats(q, q_row_stride, k_pages, v_pages, block_table, table_width, seq_of_token, positions, out,
+                                                            n_tokens, n_heads, n_kv, head_dim, value_dim, page_size, scale, sinks, stats, dtype, stream);
+    if (rc) return rc;
+    const Weighed w{weights, slots, nullptr, n_slots, places, 0};
+    if (!float_takes(q, q_row_stride, k_pages, head_dim, dtype)) {
+        if (dtype == SIA_F32)
+            return weigh_plain((const float*)q, q_row_stride, (const float*)k_pages, block_table, table_width, cu_q, kv_len, stats, n_seqs, max_kv, n_heads,
+                               n_kv, head_dim, page_size, n_pages, scale, w, stream);
+        return weigh_plain((const bf16_t*)q, q_row_stride, (const bf16_t*)k_pages, block_table, table_width, cu_q, kv_len, stats, n_seqs, max_kv, n_heads, n_kv,
+                           head_dim, page_size, n_pages, scale, w, stream);
+    }
+    const Cut cut = cut_float(n_tokens, q_bound, n_seqs, max_kv, n_heads, n_kv, head_dim);
+    float* parts = cut.floats ? stats + (long long)n_tokens * n_heads : nullptr;
+#define OF_SIZE(T, DP)                                                                                                                                  \
+    weigh_float<T, DP>((const T*)q, q_row_stride, (const T*)k_pages, block_table, table_width, cu_q, kv_len, stats, parts, n_seqs, max_kv, n_heads, n_kv, \
+                       head_dim, page_size, n_pages, scale, cut, w, stream)
+#define OF_TYPE(T) (head_dim <= 32 ? OF_SIZE(T, 32) : head_dim <= 64 ? OF_SIZE(T, 64) : head_dim <= 128 ? OF_SIZE(T, 128) : OF_SIZE(T, 256))
+    return dtype == SIA_F32 ? OF_TYPE(float) : OF_TYPE(bf16_t);
+#undef OF_TYPE
+#undef OF_SIZE
 }

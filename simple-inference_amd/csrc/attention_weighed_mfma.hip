@@ -397,70 +397,87 @@ static int shares_of(int group) {
 
 SIA_EXPORT int sia_attn_weighed_max_group() { return JOIN_MOST_HEADS; }
 
-// Floats that sia_attn_weighed_decode's workspace holds.
-SIA_EXPORT long long sia_attn_weighed_decode_workspace(int n_seqs, int n_heads, int max_kv) {
-    if (n_seqs <= 0 || n_heads <= 0 || max_kv <= 0) return 0;
-    return (long long)n_seqs * n_heads * (row_keys_of(max_kv) + (long long)splits_of(max_kv) * (HD + 2));
+// Floats of the single tokens' workspace: scores, and the splits' states.
+static long long single_floats(int n_single, int n_heads, int max_kv) {
+    return n_single <= 0 ? 0 : (long long)n_single * n_heads * (row_keys_of(max_kv) + (long long)splits_of(max_kv) * (HD + 2));
 }
 
-// Sequences 0 .. n_seqs-1 of the step, each with one new token, which is row s of q, and none longer than max_kv; weights [n_slots][n_kv]
-// [places], a sequence's row at slots[s].
-SIA_EXPORT int sia_attn_weighed_decode(const void* q, int q_row_stride, const void* k_pages, const void* v_pages, const int* block_table,
-                                       int table_width, const int* cu_q, const int* kv_len, void* out, float* ws, int n_seqs, int n_heads, int n_kv,
-                                       int page_size, float scale, const float* sinks, int max_kv, float* weights, const int* slots, int n_slots,
-                                       int places, hipStream_t stream) {
-    if (n_seqs <= 0) return 0;
-    const int ps_log2 = log2_of(page_size);
-    if (ps_log2 < 3 || n_kv <= 0 || n_heads % n_kv || n_heads / n_kv > JOIN_MOST_HEADS || n_heads > 65535 || n_seqs > 65535 || q_row_stride % 8 || table_width <= 0 ||
-        max_kv <= 0 || places < max_kv || n_slots <= 0 || !ws || !weights || !(scale > 0.f))
-        return SIA_BAD_ARGUMENT;
+static int attend_single(const bf16_t* q, int q_row_stride, const bf16_t* k_pages, const bf16_t* v_pages, const int* block_table, int table_width,
+                         const int* cu_q, const int* kv_len, bf16_t* out, float* ws, int n_single, int n_heads, int n_kv, int ps_log2, float scale,
+                         const float* sinks, int max_kv, Weighed w, hipStream_t stream) {
     const int share = shares_of(n_heads / n_kv), n_groups = n_kv * share, max_splits = splits_of(max_kv);
-    const Weighed w{weights, slots, ws, n_slots, places, (int)row_keys_of(max_kv)};
+    w.scores = ws;
+    w.row_keys = (int)row_keys_of(max_kv);
     const int most_keys = (int)min((long long)max_kv, (long long)table_width << ps_log2);      // what there is room for, whatever kv_len says
-    float* acc = ws + (long long)n_seqs * n_heads * w.row_keys;
-    float* ml = acc + (long long)n_seqs * n_heads * max_splits * HD;
+    float* acc = ws + (long long)n_single * n_heads * w.row_keys;
+    float* ml = acc + (long long)n_single * n_heads * max_splits * HD;
     const size_t lds_bytes = (size_t)DEC_WAVES * (n_heads / n_groups) * (HD + 2) * sizeof(float);
-    hipLaunchKernelGGL(weighed_decode_kernel, dim3(n_groups, n_seqs, max_splits), dim3(DEC_WAVES * SIA_WAVE), lds_bytes, stream, (const bf16_t*)q,
-                       q_row_stride, (const bf16_t*)k_pages, (const bf16_t*)v_pages, block_table, table_width, cu_q, kv_len, acc, ml, (bf16_t*)out,
-                       n_heads, n_groups, ps_log2, scale, sinks, max_splits, share, most_keys, w);
+    hipLaunchKernelGGL(weighed_decode_kernel, dim3(n_groups, n_single, max_splits), dim3(DEC_WAVES * SIA_WAVE), lds_bytes, stream, q, q_row_stride,
+                       k_pages, v_pages, block_table, table_width, cu_q, kv_len, acc, ml, out, n_heads, n_groups, ps_log2, scale, sinks, max_splits,
+                       share, most_keys, w);
     if (max_splits > 1 || share > 1)
-        hipLaunchKernelGGL(weighed_join_kernel, dim3(n_kv, n_seqs, n_heads / n_kv + (max_kv + JOIN_KEYS - 1) / JOIN_KEYS), dim3(JOIN_KEYS), 0, stream, acc, ml,
-                           cu_q, kv_len, (bf16_t*)out, n_heads, n_kv, max_splits, share, sinks, most_keys, w);
+        hipLaunchKernelGGL(weighed_join_kernel, dim3(n_kv, n_single, n_heads / n_kv + (max_kv + JOIN_KEYS - 1) / JOIN_KEYS), dim3(JOIN_KEYS), 0,
+                           stream, acc, ml, cu_q, kv_len, out, n_heads, n_kv, max_splits, share, sinks, most_keys, w);
     return SIA_LAUNCH_CHECK();
 }
 
 // How the runs of a launch are cut.  Two workgroups are on a compute unit at a time: 512 in all.
-static Cut cut_of(int total_tokens, int q_bound, int n_runs, int max_kv, int n_heads, int n_kv) {
-    return cut_runs(total_tokens, q_bound, n_runs, max_kv, n_heads / n_kv, n_kv, RUN_KEYS, 64, 512);
+static Cut cut_of(int run_tokens, int q_bound, int n_runs, int run_kv, int n_heads, int n_kv) {
+    return cut_runs(run_tokens, q_bound, n_runs, run_kv, n_heads / n_kv, n_kv, RUN_KEYS, 64, 512);
 }
 
-// Floats of sia_weigh_runs' workspace (0: none).
-SIA_EXPORT long long sia_weigh_runs_workspace(int total_tokens, int q_bound, int n_runs, int max_kv, int n_heads, int n_kv) {
-    if (total_tokens <= 0 || q_bound <= 0 || n_runs <= 0 || max_kv <= 0 || n_kv <= 0 || n_heads % n_kv) return 0;
-    return cut_of(total_tokens, q_bound, n_runs, max_kv, n_heads, n_kv).floats;
-}
-
-// Sequences seq_begin .. seq_end-1, total_tokens tokens in all, none with more than q_bound tokens and max_kv places.
-SIA_EXPORT int sia_weigh_runs(const void* q, int q_row_stride, const void* k_pages, const int* block_table, int table_width, const int* cu_q,
-                              const int* kv_len, const float* row_stats, float* ws, int seq_begin, int seq_end, int total_tokens, int q_bound, int n_heads,
-                              int n_kv, int page_size, float scale, int max_kv, float* weights, const int* slots, int n_slots, int places,
-                              hipStream_t stream) {
-    if (seq_end <= seq_begin || total_tokens <= 0 || q_bound <= 0) return 0;
-    const int ps_log2 = log2_of(page_size), n_runs = seq_end - seq_begin;
-    if (ps_log2 < 3 || n_kv <= 0 || n_heads % n_kv || n_runs > 65535 || q_row_stride % 8 || table_width <= 0 || max_kv <= 0 || places < max_kv ||
-        n_slots <= 0 || !row_stats || !weights || (long long)q_bound * (n_heads / n_kv) > 0x7fffff00)
-        return SIA_BAD_ARGUMENT;
-    const Cut cut = cut_of(total_tokens, q_bound, n_runs, max_kv, n_heads, n_kv);
-    const int blocks = (max_kv + RUN_KEYS - 1) / RUN_KEYS;
-    if (cut.most_work > 65535 || blocks > 65535 || (cut.floats && !ws)) return SIA_BAD_ARGUMENT;
-    const Weighed w{weights, slots, nullptr, n_slots, places, 0};
-    const int most_keys = (int)min((long long)max_kv, (long long)table_width << ps_log2);
-    float* parts = cut.floats ? ws : nullptr;
-    hipLaunchKernelGGL(weigh_runs_kernel, dim3(n_kv, cut.most_work, n_runs), dim3(RUN_THREADS), 0, stream, (const bf16_t*)q, q_row_stride,
-                       (const bf16_t*)k_pages, block_table, table_width, cu_q, kv_len, row_stats, n_heads, n_kv, ps_log2, scale, seq_begin,
-                       cut.chunk_rows, most_keys, parts, w);
+static int weigh_runs(const bf16_t* q, int q_row_stride, const bf16_t* k_pages, const int* block_table, int table_width, const int* cu_q,
+                      const int* kv_len, const float* row_stats, float* parts, int seq_begin, int n_runs, const Cut& cut, int n_heads, int n_kv,
+                      int ps_log2, float scale, int run_kv, const Weighed& w, hipStream_t stream) {
+    const int blocks = (run_kv + RUN_KEYS - 1) / RUN_KEYS, most_keys = (int)min((long long)run_kv, (long long)table_width << ps_log2);
+    hipLaunchKernelGGL(weigh_runs_kernel, dim3(n_kv, cut.most_work, n_runs), dim3(RUN_THREADS), 0, stream, q, q_row_stride, k_pages, block_table,
+                       table_width, cu_q, kv_len, row_stats, n_heads, n_kv, ps_log2, scale, seq_begin, cut.chunk_rows, most_keys, parts, w);
     if (parts)
         hipLaunchKernelGGL(weigh_add_kernel<RUN_KEYS>, dim3(n_kv, blocks, n_runs), dim3(RUN_KEYS), 0, stream, parts, cu_q, kv_len, n_heads, n_kv,
                            seq_begin, cut.chunk_rows, most_keys, cut.most_work, w);
     return SIA_LAUNCH_CHECK();
+}
+
+extern "C" int sia_attn_prefill_stats(const void*, int, const void*, const void*, const int*, int, const int*, const int*, void*, int, int, int, int,
+                                      int, int, int, int, int, int, float, const float*, float*, hipStream_t);
+
+// Floats that sia_attn_weighed's workspace holds (arguments as there).
+SIA_EXPORT long long sia_attn_weighed_workspace(int n_single, int n_seqs, int n_tokens, int q_bound, int run_kv, int max_kv, int n_heads, int n_kv) {
+    if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || max_kv <= 0) return 0;
+    long long floats = single_floats(n_single, n_heads, max_kv);
+    if (n_single < n_seqs && q_bound > 0 && run_kv > 0)
+        floats += (long long)n_tokens * n_heads + cut_of(n_tokens - n_single, q_bound, n_seqs - n_single, run_kv, n_heads, n_kv).floats;
+    return floats;
+}
+
+// Sequences 0 .. n_single-1 of the step bring one token each, which is row s of q, and none is longer than max_kv; sequences n_single .. n_seqs-1
+// bring at most q_bound tokens over at most run_kv places, n_tokens - n_single in all, in row tiles as sia_attn_prefill counts them.  weights
+// [n_slots][n_kv][places], a sequence's row at slots[s].
+SIA_EXPORT int sia_attn_weighed(const void* q, int q_row_stride, const void* k_pages, const void* v_pages, const int* block_table, int table_width,
+                                const int* cu_q, const int* kv_len, void* out, float* ws, int n_single, int n_seqs, int n_tokens, int n_tiles,
+                                int n_tiles_split, int n_tiles_long, int q_bound, int run_kv, int max_kv, int n_heads, int n_kv, int page_size,
+                                float scale, const float* sinks, float* weights, const int* slots, int n_slots, int places, hipStream_t stream) {
+    if (n_seqs <= 0 || n_tokens <= 0) return 0;
+    const int ps_log2 = log2_of(page_size), n_runs = n_seqs - n_single;
+    const bool runs = n_runs > 0 && q_bound > 0 && n_tokens > n_single;
+    if (ps_log2 < 3 || n_kv <= 0 || n_heads % n_kv || n_heads / n_kv > JOIN_MOST_HEADS || n_heads > 65535 || n_seqs > 65535 || n_single < 0 || n_runs < 0 ||
+        q_row_stride % 8 || table_width <= 0 || max_kv <= 0 || places < max_kv || n_slots <= 0 || !ws || !weights || !(scale > 0.f) ||
+        (runs && (run_kv <= 0 || run_kv > max_kv || (long long)q_bound * (n_heads / n_kv) > 0x7fffff00)))
+        return SIA_BAD_ARGUMENT;
+    const Cut cut = runs ? cut_of(n_tokens - n_single, q_bound, n_runs, run_kv, n_heads, n_kv) : Cut{};
+    if (runs && (cut.most_work > 65535 || (run_kv + RUN_KEYS - 1) / RUN_KEYS > 65535)) return SIA_BAD_ARGUMENT;
+    const Weighed w{weights, slots, nullptr, n_slots, places, 0};
+    if (n_single > 0) {
+        const int rc = attend_single((const bf16_t*)q, q_row_stride, (const bf16_t*)k_pages, (const bf16_t*)v_pages, block_table, table_width, cu_q, kv_len,
+                                     (bf16_t*)out, ws, n_single, n_heads, n_kv, ps_log2, scale, sinks, max_kv, w, stream);
+        if (rc) return rc;
+    }
+    if (!runs) return 0;
+    float* stats = ws + single_floats(n_single, n_heads, max_kv);
+    float* parts = cut.floats ? stats + (long long)n_tokens * n_heads : nullptr;
+    const int rc = sia_attn_prefill_stats(q, q_row_stride, k_pages, v_pages, block_table, table_width, cu_q, kv_len, out, n_single, n_seqs, n_tiles,
+                                          n_tiles_split, n_tiles_long, q_bound, run_kv, n_heads, n_kv, page_size, scale, sinks, stats, stream);
+    if (rc) return rc;
+    return weigh_runs((const bf16_t*)q, q_row_stride, (const bf16_t*)k_pages, block_table, table_width, cu_q, kv_len, stats, parts, n_single, n_runs, cut,
+                      n_heads, n_kv, ps_log2, scale, run_kv, w, stream);
 }

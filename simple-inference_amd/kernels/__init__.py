@@ -109,16 +109,10 @@ _SIGNATURES = {
                           _c_ptr, _c_float, _c_int, _c_ptr],
     "sia_attention_max_head_dim": [],
     "sia_attention_generic_max_head_dim": [],
-    "sia_attention_generic_stats": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int,
-                                    _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_ptr, _c_int, _c_ptr],
-    "sia_weigh_plain": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
-                        _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_ptr],
-    "sia_attention_f32_stats": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
-                                _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_ptr, _c_ptr],
-    "sia_weigh_float_takes": [_c_int],
-    "sia_weigh_float_workspace": [_c_int] * 7,
-    "sia_weigh_float": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
-                        _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_int, _c_ptr],
+    "sia_attention_weighed_workspace": [_c_int] * 7,
+    "sia_attention_weighed": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int,
+                              _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_ptr, _c_ptr, _c_int,
+                              _c_int, _c_int, _c_ptr],
     "sia_rope_axes_max": [],
     "sia_rope_axes_kv_write": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int,
                                _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr],
@@ -219,9 +213,6 @@ _ATTN_SIGNATURES = {
     "sia_attn_prefill_forms": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr,
                                _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float,
                                _c_int, _c_int, _c_ptr, _c_float, _c_int, _c_ptr],
-    "sia_attn_prefill_stats": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr,
-                               _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float,
-                               _c_ptr, _c_ptr, _c_ptr],
     "sia_attn_decode_walk": [_c_int, _c_int, _c_int],
     "sia_attn_mfma_forms": [],
     "sia_attn_decode_max_splits": [_c_int, _c_int],
@@ -237,12 +228,9 @@ _ATTN_SIGNATURES = {
 # of the libraries without the forms
 _WEIGHED_SIGNATURES = {
     "sia_attn_weighed_max_group": [],
-    "sia_attn_weighed_decode_workspace": [_c_int, _c_int, _c_int],
-    "sia_attn_weighed_decode": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int,
-                                _c_int, _c_float, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
-    "sia_weigh_runs_workspace": [_c_int] * 6,
-    "sia_weigh_runs": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int,
-                       _c_int, _c_int, _c_float, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
+    "sia_attn_weighed_workspace": [_c_int] * 8,
+    "sia_attn_weighed": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int,
+                         _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
 }
 
 
@@ -355,7 +343,7 @@ class HipKernels:
         self.core.sia_delta_rule_workspace.restype = ctypes.c_longlong
         self.core.sia_linear_unit_workspace.restype = ctypes.c_longlong
         self.core.sia_bonus_recurrence_workspace.restype = ctypes.c_longlong
-        self.core.sia_evict_workspace.restype = self.core.sia_weigh_float_workspace.restype = ctypes.c_longlong
+        self.core.sia_evict_workspace.restype = self.core.sia_attention_weighed_workspace.restype = ctypes.c_longlong
         self.tiled_experts = True        # many slots in bfloat16: experts' products on the matrix cores, slots sorted by expert
         self._attn_libs = {}
         # the short way to the current stream's handle, where this torch has it (a few microseconds less a launch)
@@ -432,9 +420,10 @@ class HipKernels:
             lib.sia_attn_decode_workspace.restype = ctypes.c_longlong
             if not forms:
                 _bind(lib, _WEIGHED_SIGNATURES)
-                lib.sia_attn_weighed_decode_workspace.restype = lib.sia_weigh_runs_workspace.restype = ctypes.c_longlong
+                lib.sia_attn_weighed_workspace.restype = ctypes.c_longlong
             if lib.sia_attn_mfma_head_dim() != head_dim or bool(lib.sia_attn_mfma_forms()) != forms:
                 raise KernelError(f"library {name} was built for another head size or other forms")
+            lib.prefill_rows = (lib.sia_attn_prefill_rows(), lib.sia_attn_prefill_rows_split(), lib.sia_attn_prefill_rows_long())
             self._attn_libs[(head_dim, forms)] = lib
         return lib
 
@@ -2099,60 +2088,29 @@ class HipKernels:
         out = qkv.new_empty((n, n_heads * value_dim))
         if not n:
             return out
-        table, pages, page = cache.block_table, cache.k_pages.shape[0], cache.page_size
+        page, n_single, stream = cache.page_size, ctx.n_decode_seqs, self._stream_here()
+        (slots, _, places), table_width = weights.shape, cache.block_table.shape[1]
+        given = (qkv.data_ptr(), width, cache.k_pages.data_ptr(), cache.v_pages.data_ptr(), cache.block_table.data_ptr(), table_width)
         if (self.use_mfma_attention and qkv.dtype == torch.bfloat16 and head_dim % 16 == 0 and head_dim <= 256 and value_dim == head_dim
                 and page >= 8 and page & (page - 1) == 0 and width % 8 == 0 and scale > 0 and n_heads // n_kv_heads <= 256
                 and _in_pieces(qkv, cache.k_pages, cache.v_pages)):
-            self._weighed_mfma(qkv, out, n_heads, n_kv_heads, head_dim, float(scale), ctx, cache, sinks, weights, max_kv)
+            # single tokens by one walk over keys and values, runs by the attention kernel and the scores once more
+            lib = self._attn_lib(head_dim)
+            tiles, q_bound, run_kv = self._run_tiles(lib, ctx) if n_single < ctx.n_seqs else ((0, 0, 0), 0, 0)
+            ws = weights.new_empty((lib.sia_attn_weighed_workspace(n_single, ctx.n_seqs, n, q_bound, run_kv, max_kv, n_heads, n_kv_heads),))
+            self._check(lib.sia_attn_weighed(
+                *given, ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), out.data_ptr(), ws.data_ptr(), n_single, ctx.n_seqs, n, *tiles, q_bound,
+                run_kv, max_kv, n_heads, n_kv_heads, page, float(scale), _ptr(sinks), weights.data_ptr(), ctx.state_slots.data_ptr(), slots,
+                places, stream), "attn_weighed")
             return out
-        stats = weights.new_empty((n, n_heads))
-        stream, places = self._stream_here(), (weights.shape[0], weights.shape[2])
-        if qkv.dtype == torch.float32:
-            self._check(self.core.sia_attention_f32_stats(
-                _ptr(qkv), width, _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(table), table.shape[1], _ptr(ctx.seq_of_token),
-                _ptr(ctx.positions), _ptr(out), n, ctx.n_decode_seqs, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim, value_dim, page,
-                float(scale), _ptr(sinks), _ptr(stats), stream), "attention_f32_stats")
-        else:
-            self._check(self.core.sia_attention_generic_stats(
-                _ptr(qkv), width, _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(table), table.shape[1], _ptr(ctx.seq_of_token),
-                _ptr(ctx.positions), _ptr(out), n, n_heads, n_kv_heads, head_dim, value_dim, page, float(scale), _ptr(sinks), _ptr(stats),
-                _DT[qkv.dtype], stream), "attention_generic_stats")
-        weigh = (_ptr(qkv), width, _ptr(cache.k_pages), _ptr(table), table.shape[1], _ptr(ctx.cu_q), _ptr(ctx.kv_len),
-                 _ptr(ctx.state_slots), _ptr(stats), _ptr(weights), *places, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim, page,
-                 pages, float(scale))
-        if self.core.sia_weigh_float_takes(head_dim) and width % 4 == 0 and _in_pieces(qkv, cache.k_pages):
-            q_bound = max(ctx.q_lens)
-            floats = self.core.sia_weigh_float_workspace(n, q_bound, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim)
-            ws = weights.new_empty((floats,)) if floats else None
-            self._check(self.core.sia_weigh_float(*weigh, n, q_bound, _ptr(ws), _DT[qkv.dtype], stream), "weigh_float")
-        else:
-            self._check(self.core.sia_weigh_plain(*weigh, _DT[qkv.dtype], stream), "weigh_plain")
+        q_bound = max(ctx.q_lens)
+        ws = weights.new_empty((self.core.sia_attention_weighed_workspace(n, q_bound, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim),))
+        self._check(self.core.sia_attention_weighed(
+            *given, ctx.seq_of_token.data_ptr(), ctx.positions.data_ptr(), ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), out.data_ptr(),
+            ws.data_ptr(), n, n_single, ctx.n_seqs, q_bound, max_kv, n_heads, n_kv_heads, head_dim, value_dim, page, cache.k_pages.shape[0],
+            float(scale), _ptr(sinks), weights.data_ptr(), ctx.state_slots.data_ptr(), slots, places, _DT[qkv.dtype], stream),
+            "attention_weighed")
         return out
-
-    def _weighed_mfma(self, qkv, out, n_heads, n_kv, head_dim, scale, ctx, cache, sinks, weights, max_kv):
-        """Single tokens by one walk over keys and values, runs by the attention kernel and the scores once more."""
-        lib, n_dec, page, stream = self._attn_lib(head_dim), ctx.n_decode_seqs, cache.page_size, self._stream_here()
-        (slots, _, places), (table_width, width) = weights.shape, (cache.block_table.shape[1], qkv.shape[1])
-        q, k, v, table = qkv.data_ptr(), cache.k_pages.data_ptr(), cache.v_pages.data_ptr(), cache.block_table.data_ptr()
-        cu_q, kv_len, sums, rows = ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), weights.data_ptr(), ctx.state_slots.data_ptr()
-        if n_dec:
-            ws = weights.new_empty((lib.sia_attn_weighed_decode_workspace(n_dec, n_heads, max_kv),))
-            self._check(lib.sia_attn_weighed_decode(
-                q, width, k, v, table, table_width, cu_q, kv_len, out.data_ptr(), ws.data_ptr(), n_dec, n_heads, n_kv, page, scale,
-                _ptr(sinks), max_kv, sums, rows, slots, places, stream), "attn_weighed_decode")
-        if n_dec >= ctx.n_seqs:
-            return
-        stats = weights.new_empty((ctx.n_tokens, n_heads))
-        tiles, q_bound, kv_bound = self._run_tiles(lib, ctx)
-        self._check(lib.sia_attn_prefill_stats(
-            q, width, k, v, table, table_width, cu_q, kv_len, out.data_ptr(), n_dec, ctx.n_seqs, *tiles, q_bound, kv_bound, n_heads, n_kv,
-            page, scale, _ptr(sinks), stats.data_ptr(), stream), "attn_prefill_stats")
-        tokens = ctx.n_tokens - n_dec
-        floats = lib.sia_weigh_runs_workspace(tokens, q_bound, ctx.n_seqs - n_dec, kv_bound, n_heads, n_kv)
-        ws = weights.new_empty((floats,)) if floats else None
-        self._check(lib.sia_weigh_runs(
-            q, width, k, table, table_width, cu_q, kv_len, stats.data_ptr(), _ptr(ws), n_dec, ctx.n_seqs, tokens, q_bound, n_heads, n_kv,
-            page, scale, kv_bound, sums, rows, slots, places, stream), "weigh_runs")
 
     def evict_cache(self, ctx, cache, budget, keep_first=0, keep_last=0):
         """Drops what got least attention: every sequence of the step with more than ``budget`` places (``ctx.kv_len``) keeps, for
@@ -2190,8 +2148,7 @@ class HipKernels:
     def _run_tiles(lib, ctx):
         """Row tiles of the step's runs at each of the prefill kernel's workgroup sizes, and the most tokens and keys of one."""
         runs = ctx.q_lens[ctx.n_decode_seqs:]
-        tiles = tuple(sum(-(-q // rows) for q in runs) if rows else 0
-                      for rows in (lib.sia_attn_prefill_rows(), lib.sia_attn_prefill_rows_split(), lib.sia_attn_prefill_rows_long()))
+        tiles = tuple(sum(-(-q // rows) for q in runs) if rows else 0 for rows in lib.prefill_rows)
         return tiles, int(max(runs)), int(getattr(ctx, "max_run_kv_len", 0) or ctx.max_kv_len)
 
     def _attention_plan(self, lib, device, n_heads, n_kv_heads, head_dim, window, ctx, chunk=0, keep_first=0, page_size=0):
