@@ -40,22 +40,24 @@ __device__ __forceinline__ int lanes_upto(int v) {
     return v;
 }
 
-// What a wave's value `v` adds up to over the waves before this one, and over all; scratch: SELECT_WAVES ints.
-__device__ __forceinline__ int waves_before(int v, int* scratch, int& total) {
-    const int lane = threadIdx.x % SIA_WAVE, wave = threadIdx.x / SIA_WAVE;
-    if (lane == 0) scratch[wave] = v;
-    __syncthreads();
-    int before = 0;
-    total = 0;
+// What the waves' values (the same in all of a wave's lanes) add up to over the waves before this one.  leave, a barrier, then before; nobody may
+// still be reading the row of scratch.
+__device__ __forceinline__ void leave(int v, int* scratch) {
+    if (threadIdx.x % SIA_WAVE == 0) scratch[threadIdx.x / SIA_WAVE] = v;
+}
+__device__ __forceinline__ int before(const int* scratch, int& all) {
+    const int wave = threadIdx.x / SIA_WAVE;
+    int sum = 0;
+    all = 0;
 #pragma unroll
     for (int w = 0; w < SELECT_WAVES; ++w) {
         const int x = scratch[w];
-        before += w < wave ? x : 0;
-        total += x;
+        sum += w < wave ? x : 0;
+        all += x;
     }
-    __syncthreads();
-    return before;
+    return sum;
 }
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(lanes_upto(v), SIA_WAVE - 1); }
 
 // HELD: places of a wave's stretch that a lane keeps the keys of (64 HELD places a wave); 0: stretches of any length, read again every time.
 template <int HELD>
@@ -63,9 +65,9 @@ __global__ __launch_bounds__(SELECT_THREADS) void evict_select_kernel(
     const float* __restrict__ weights, const int* __restrict__ slots, const int* __restrict__ kv_len, int n_slots, int places, int max_kv,
     int n_kv, int budget, int keep_first, int keep_last, int max_moves, int* __restrict__ kept, int* __restrict__ lengths,
     int* __restrict__ from, int* __restrict__ to, int2* __restrict__ n_moves) {
-    __shared__ int bins[COPIES][BINS];
-    __shared__ int scratch[SELECT_WAVES];
-    __shared__ uint32_t found[2];      // the largest digit that enough places reach; how many of those that have it are still wanted
+    __shared__ int bins[COPIES + 2][BINS];      // of the first digit in copies, of the others
+    __shared__ int scratch[7][SELECT_WAVES];    // a row for everything that crosses the waves
+    __shared__ uint32_t found[3][2];      // the largest digit that enough places reach; how many of those that have it are still wanted
     const int hk = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid % SIA_WAVE, wave = tid / SIA_WAVE;
     const size_t unit = (size_t)seq * n_kv + hk;
     const int slot = slots[seq], length = max(0, min(kv_len[seq], min(max_kv, places)));
@@ -83,6 +85,8 @@ __global__ __launch_bounds__(SELECT_THREADS) void evict_select_kernel(
     to += unit * max_moves;
     // the wave's stretch of the places below hi, 64 of them a step
     const int steps = HELD ? HELD : (hi + SELECT_THREADS - 1) / SELECT_THREADS, begin = wave * steps * SIA_WAVE;
+#pragma unroll
+    for (int c = 0; c < COPIES + 2; ++c) reinterpret_cast<int2*>(bins[c])[tid] = make_int2(0, 0);
     uint32_t held[HELD ? HELD : 1];
     auto load_key = [&](int j) { return j >= lo && j < hi ? order_key(w[j]) : 0u; };      // no place has the key 0: minus infinity has more
     if constexpr (HELD != 0) {
@@ -104,38 +108,39 @@ __global__ __launch_bounds__(SELECT_THREADS) void evict_select_kernel(
     };
     uint32_t digits = 0;
     int left = wanted;
+    __syncthreads();
     if (wanted > 0) {
 #pragma unroll
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, mask = pass == 2 ? 1023 : 2047;
 #pragma unroll
-            for (int c = 0; c < COPIES; ++c) reinterpret_cast<int2*>(bins[c])[tid] = make_int2(0, 0);
-            __syncthreads();
-#pragma unroll
             for (int e = 0; e < steps; ++e) {
                 const uint32_t key = key_at(e);
-                if (key != 0 && (pass == 0 || key >> (pass == 1 ? 21 : 10) == digits)) atomicAdd(&bins[lane % COPIES][(key >> shift) & mask], 1);
+                if (key != 0 && (pass == 0 || key >> (pass == 1 ? 21 : 10) == digits))
+                    atomicAdd(&bins[pass == 0 ? lane % COPIES : COPIES - 1 + pass][(key >> shift) & mask], 1);
             }
             __syncthreads();
             // threads take two bins each, from the top
             int2 two = make_int2(0, 0);
 #pragma unroll
-            for (int c = 0; c < COPIES; ++c) {
-                const int2 own = reinterpret_cast<const int2*>(bins[c])[BINS / 2 - 1 - tid];
+            for (int c = 0; c < (pass == 0 ? COPIES : 1); ++c) {
+                const int2 own = reinterpret_cast<const int2*>(bins[pass == 0 ? c : COPIES - 1 + pass])[BINS / 2 - 1 - tid];
                 two.x += own.x;
                 two.y += own.y;
             }
             const int upto = lanes_upto(two.x + two.y);
-            int total;
-            const int above = waves_before(__builtin_amdgcn_readlane(upto, SIA_WAVE - 1), scratch, total) + upto - two.x - two.y;
+            int all;
+            leave(__builtin_amdgcn_readlane(upto, SIA_WAVE - 1), scratch[pass]);
+            __syncthreads();
+            const int above = before(scratch[pass], all) + upto - two.x - two.y;
             if (above < left && above + two.x + two.y >= left) {
                 const bool upper = above + two.y >= left;
-                found[0] = BINS - 1 - 2 * tid - (upper ? 0 : 1);
-                found[1] = left - (upper ? above : above + two.y);
+                found[pass][0] = BINS - 1 - 2 * tid - (upper ? 0 : 1);
+                found[pass][1] = left - (upper ? above : above + two.y);
             }
             __syncthreads();
-            digits = digits << (pass == 2 ? 10 : 11) | found[0];
-            left = found[1];
+            digits = digits << (pass == 2 ? 10 : 11) | found[pass][0];
+            left = found[pass][1];
         }
     }
     // keys above `digits` are kept, and of those equal to it the `left` lowest places (with nothing wanted: none of a key that there is not)
@@ -153,8 +158,10 @@ __global__ __launch_bounds__(SELECT_THREADS) void evict_select_kernel(
         beyond += over && j >= edge;
         near += over && j >= edge && j < budget;
     }
-    int total;
-    const int ties_before = waves_before(ties, scratch, total);
+    int all;
+    leave(ties, scratch[3]);
+    __syncthreads();
+    const int ties_before = before(scratch[3], all);
     const unsigned long long below = (1ull << lane) - 1;
     // of the ties, those with fewer than `left` before them: where they lie matters to the counts only if the wave has some of them and some not
     const int ties_kept = min(max(left - ties_before, 0), ties);
@@ -176,13 +183,14 @@ __global__ __launch_bounds__(SELECT_THREADS) void evict_select_kernel(
     }
     // the wave's holes: its places below the edge that nothing stays at
     const int reach = steps * SIA_WAVE, upper = min(max(edge - begin, 0), reach);
-    const int packed_stay = __builtin_amdgcn_readlane(lanes_upto(stay), SIA_WAVE - 1);
-    int all_movers, all_near;
-    int holes = waves_before(upper - packed_stay, scratch, total);
-    int movers = waves_before(__builtin_amdgcn_readlane(lanes_upto(beyond), SIA_WAVE - 1), scratch, all_movers);
-    waves_before(__builtin_amdgcn_readlane(lanes_upto(near), SIA_WAVE - 1), scratch, all_near);
-    total = min(all_movers, max_moves);
-    if (tid == 0) n_moves[unit] = make_int2(all_near, total);
+    leave(upper - wave_total(stay), scratch[4]);
+    leave(wave_total(beyond), scratch[5]);
+    leave(wave_total(near), scratch[6]);
+    __syncthreads();
+    int holes = before(scratch[4], all), all_movers, movers = before(scratch[5], all_movers);
+    before(scratch[6], all);
+    const int total = min(all_movers, max_moves);
+    if (tid == 0) n_moves[unit] = make_int2(all, total);
     // then the lists, in order
     int rank = 0;
 #pragma unroll
