@@ -24,12 +24,11 @@ __device__ __forceinline__ void add_weights(float* __restrict__ row, const float
     }
 }
 
-#ifndef WT
-#define WT 8
-#endif
 // Workgroups of four waves that share one (sequence, key/value head) with n_tiles tiles: the largest power of two that leaves each WEIGHED_TILES.  A
-// function of the sequence's own length only.
-constexpr int WEIGHED_TILES = WT, WEIGHED_MAX_SPLITS = 64;
+// function of the sequence's own length only.  us a call with 4, 8, 16 and 32 tiles a split: one row over 2,048 keys, 32 heads of 128 on 8: 9.4 9.7 11.8 16.3;
+// 27 of 24 over about 700 28.9 25.4 31.4 25.1;  8 of 24 over 2,048 25.9 19.2 18.2 19.5;  3 of 32 over 12,000 44.8 42.5 43.8 42.6;  4 of 16 on 1 over
+// 6,000 14.0 15.7 19.0 26.6;  64 of 32 over about 900 81.0 70.1 69.7 64.2.
+constexpr int WEIGHED_TILES = 8, WEIGHED_MAX_SPLITS = 64;
 __host__ __device__ inline int weighed_splits(int n_tiles) {
     int s = 1;
     while (s < WEIGHED_MAX_SPLITS && 2 * s * WEIGHED_TILES <= n_tiles) s *= 2;
@@ -57,7 +56,9 @@ __device__ __forceinline__ void clear_values(Stage& st, int kb, int g, int last)
     }
 }
 
-// grid (groups of query heads, sequences, splits), four waves of a run of tiles each, as attn_decode_kernel's plain mode.
+// grid (groups of query heads, sequences, splits), four waves of a run of tiles each, as attn_decode_kernel's plain mode.  The memory bounds it:  8 rows over
+// 2,048 keys, 24 heads of 128 on 8, 15.1 us and 3.9 for the join (67 MB: 4.4 TB/s), 3 of 32 over 12,000 37.6 and 5.4 (150 MB: 4.0 TB/s).  With the keys and
+// values in the last-level cache a whole call takes 19.1 and 31.3 us, attention alone 18.7 and 29.7.
 // kv_share groups of query heads read one key/value head; with more than one, or several splits, the join makes the weights.
 __global__ __launch_bounds__(DEC_WAVES* SIA_WAVE) void weighed_decode_kernel(
     const bf16_t* __restrict__ q, int q_row_stride, const bf16_t* __restrict__ kp, const bf16_t* __restrict__ vp,
@@ -217,6 +218,9 @@ constexpr int RUN_WAVES = 4, WAVE_BLOCKS = 4, WAVE_KEYS = 16 * WAVE_BLOCKS, RUN_
 // grid (key/value heads, pieces of work of a run, runs): workgroups go to the chip's dies in turn, so that with 8 key/value heads a die reads
 // one head's keys and queries.  A wave holds its 64 keys as operands; the rows come through LDS 32 at a time, two stages of it, the next tile's loads under way while one is computed.  (Read from memory as
 // operands, 16 rows of 16 bytes a lane, every lane is an access of its own to the first-level cache: four times as many, and what bound it.)
+// What bounds it: a score costs an exponential (16 cycles a wave), a multiply-add and an add (4 each), of a tile's 1,250 cycles
+// 1,016 are the vector unit's.  2,048 tokens of 24 heads of 128 on 8: 28 us, 74 before;  beside an attention
+// of 54.  Workgroups for 256, 384, 512, 768 and 1,536 of them 34.5 33.8 28.2 32.4 35.7: two are on a unit at a time, so 512 go in one round.
 // parts: [run][piece of work][key/value head][RUN_KEYS], or null where every block has one chunk.
 constexpr int TILE_ROWS = 32, PIECES = HD / 8, ROW_STRIDE = HD + ((HD / 16) % 2 == 0 ? 16 : 0);      // as the prefill kernel's key rows
 constexpr int RUN_THREADS = RUN_WAVES * SIA_WAVE, PER_THREAD = (TILE_ROWS * PIECES + RUN_THREADS - 1) / RUN_THREADS;

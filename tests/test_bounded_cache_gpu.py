@@ -291,6 +291,9 @@ ATTENTIONS = [
     ([70, 1, 9], [300, 5, 9], 6, 2, 22, 12),                       # heads that are not in fours
     ([1, 45], [90, 200], 4, 2, 200, 16),
     ([1] * 3, [0, 3, 0], 4, 2, 64, 16),                            # sequences without places
+    ([40, 300], [17000, 301], 2, 1, 32, 64),                       # more blocks of keys than a wave has lanes
+    ([1, 3], [40, 20], 260, 1, 16, 16),                            # more query heads a key/value head than the joining kernel takes
+    ([2] * 70, [5 + i for i in range(70)], 2, 2, 64, 16),          # many short runs
     ([1], [130], 4, 4, 256, 16),
 ]
 
@@ -448,6 +451,8 @@ EVICTIONS = [
     ([5000], 2, 64, 64, 64, 2111, 4, 513),
     ([2600, 2049, 2048], 1, 256, 256, 16, 2048, 4, 1025),
     ([9], 2, 64, 64, 16, 2, 1, 1),                         # nothing between is kept
+    ([20000, 700], 1, 16, 16, 64, 9000, 3, 4000),          # more places than a workgroup's registers hold keys of
+    ([3000], 1, 8, 8, 1, 1100, 0, 3),                      # a place a page, more pages than LDS holds of the table
 ]
 
 
@@ -527,6 +532,43 @@ def test_evict_cache_refuses(hip):
     assert torch.equal(cache.k_pages, k)
 
 
+def test_native_entries_refuse(hip):
+    """What the wrappers check first, once more where nothing is launched for it."""
+    bad, core, lib = 10001, hip.core, hip._attn_lib(64)
+    ctx, cache = Ctx([1], [40]), Cache([40], 2, 16, 64, torch.bfloat16)
+    ws, out, ints = torch.zeros(1 << 20, device=DEV), torch.zeros(1 << 16, device=DEV), torch.zeros(1 << 16, dtype=torch.int32, device=DEV)
+    k, v, w, t = (x.data_ptr() for x in (cache.k_pages, cache.v_pages, cache.weights, cache.block_table))
+    import ctypes
+
+    def rope(counts=(12, 10, 10, 0), axes=3, cycled=0, rows=10, rotary=64, page=16, dtype=1):
+        return core.sia_rope_axes_kv_write(out.data_ptr(), 512, ws.data_ptr(), ws.data_ptr(), rows, ints.data_ptr(), (ctypes.c_int * 4)(*counts), axes, cycled,
+                                           ctx.positions.data_ptr(), ctx.seq_of_token.data_ptr(), t, 3, k, v, 4, 1, 4, 2, 64, rotary, 0, page, dtype, None)
+    for change in (dict(axes=0), dict(axes=5), dict(counts=(12, 10, 9, 0)), dict(counts=(44, -6, -6, 0)), dict(rows=0), dict(rotary=65), dict(rotary=66), dict(page=0),
+                   dict(dtype=2), dict(cycled=1, counts=(0, 16, 16, 0))):
+        assert rope(**change) == bad
+
+    def evict(budget=8, first=1, last=2, max_kv=40, places=48, ws=ints.data_ptr(), dtype=1, page=16):
+        return core.sia_evict(k, v, w, ctx.state_slots.data_ptr(), ctx.kv_len.data_ptr(), t, 3, 4, 1, places, 1, max_kv, 2, 64, 64, page, budget, first, last,
+                              ints.data_ptr(), ints.data_ptr(), ws, dtype, None)
+    for change in (dict(budget=0), dict(first=-1), dict(last=-1), dict(first=7), dict(max_kv=49), dict(max_kv=60, places=60), dict(places=0), dict(ws=None),
+                   dict(dtype=3), dict(page=0)):
+        assert evict(**change) == bad
+
+    def attend(lib=lib, single=1, seqs=1, tokens=1, q_bound=0, run_kv=0, max_kv=40, heads=4, kv=2, page=16, scale=0.1, places=48, ws=ws.data_ptr()):
+        return lib.sia_attn_weighed(out.data_ptr(), 512, k, v, t, 3, ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), out.data_ptr(), ws, single, seqs, tokens, 1, 1, 1,
+                                    q_bound, run_kv, max_kv, heads, kv, page, scale, None, w, ctx.state_slots.data_ptr(), 1, places, None)
+    for change in (dict(page=12), dict(page=4), dict(heads=5), dict(scale=-1.0), dict(scale=math.nan), dict(places=39), dict(ws=None), dict(max_kv=0), dict(single=2),
+                   dict(single=0, tokens=4, q_bound=4, run_kv=41), dict(heads=514, kv=2)):
+        assert attend(**change) == bad
+
+    def plain(dim=64, vdim=64, heads=4, q_bound=1, max_kv=40, places=48, ws=ws.data_ptr(), dtype=1):
+        return core.sia_attention_weighed(out.data_ptr(), 512, k, v, t, 3, ctx.seq_of_token.data_ptr(), ctx.positions.data_ptr(), ctx.cu_q.data_ptr(),
+                                          ctx.kv_len.data_ptr(), out.data_ptr(), ws, 1, 1, 1, q_bound, max_kv, heads, 2, dim, vdim, 16, 4, 0.1, None, w,
+                                          ctx.state_slots.data_ptr(), 1, places, dtype, None)
+    for change in (dict(dim=0), dict(dim=641), dict(vdim=0), dict(vdim=641), dict(heads=3), dict(q_bound=0), dict(max_kv=49), dict(ws=None), dict(dtype=2)):
+        assert plain(**change) == bad
+
+
 # -- together --------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -578,6 +620,63 @@ def test_a_request_with_a_bounded_cache(hip, dtype):
             length = int(lengths[0])
 
 
+def test_a_bounded_cache_in_the_cache_managers_pages(hip):
+    """Two requests whose caches are cut to a budget, in pages that the cache manager hands out: pages that one gives back the other writes into, and
+    both get the bits that they get alone in pages of their own."""
+    from simple_inference_amd.cache import CacheManager
+    from simple_inference_amd.parts.context import LayerCache
+    from simple_inference_amd.parts.model import CacheLayout
+    from simple_inference_amd.parts.plan import PagedKVNeed
+    heads, kv, dim, page, budget = 4, 2, 64, 16, 64
+    cos, sin = angles(500, 32)
+    portions = {0: [100, 1, 1, 40, 1, 1, 1], 1: [30, 50, 1, 1, 60, 1, 1]}
+
+    def serve(requests):
+        layout = CacheLayout([PagedKVNeed(kv, dim, None)], [1], [(0, 0)], [], [None])
+        books = CacheManager(layout, page_size=page, num_pages=16, max_running=2, dtype=torch.bfloat16, device=DEV)
+        weights = torch.full((3, kv, 256), math.nan, device=DEV)
+        at, outs = {r: 0 for r in requests}, {r: [] for r in requests}
+        for r in requests:
+            books.admit(r)
+        for turn in range(7):
+            step = sorted(requests, key=lambda r: portions[r][turn] != 1)      # single tokens first
+            q_lens, lens = [portions[r][turn] for r in step], []
+            for r, n in zip(step, q_lens):
+                lens.append(books.extend(r, n) + n)
+            ctx = Ctx(q_lens, lens, [r for r in step])
+            tables = [books.table(0, r) for r in step]
+            width = max(len(t) for t in tables)
+            table = torch.tensor([t + [-1] * (width - len(t)) for t in tables], dtype=torch.int32, device=DEV)
+            layer = books.layer_caches([table])[0]
+            assert isinstance(layer, LayerCache) and layer.weights is None
+            layer.weights = weights
+            rows, where = [], []
+            for r, n in zip(step, q_lens):
+                rows.append(rnd(n, (heads + 2 * kv) * dim, dtype=torch.bfloat16, seed=1000 * r + at[r]))
+                t = torch.arange(at[r], at[r] + n, dtype=torch.int32)
+                where.append(torch.stack([t, t // 2, t // 3]))
+                at[r] += n
+            qkv, where = torch.cat(rows), torch.cat(where, 1).to(DEV).contiguous()
+            hip.rope_axes_kv_write(qkv, heads, kv, dim, (12, 10, 10), cos, sin, where, ctx, layer)
+            out = hip.weighed_attention(qkv, heads, kv, dim, 0.125, ctx, layer)
+            kept, _ = hip.evict_cache(ctx, layer, budget, keep_first=2, keep_last=16)
+            for s, (r, length) in enumerate(zip(step, lens)):
+                outs[r].append((out[ctx.cu_q[s]:ctx.cu_q[s + 1]].clone(), kept[s].clone()))
+                if length > budget:
+                    assert books.owns_pages(r)
+                    books.shrink(r, budget)
+            books.check()
+        return outs
+
+    both = serve([0, 1])
+    for r in (0, 1):
+        for (out, kept), (want, want_kept) in zip(both[r], serve([r])[r]):
+            # a run of tokens beside another may take another shape of workgroup: its last bits, and ties of its sums, are its own
+            if len(out) == 1:
+                assert torch.equal(kept, want_kept)
+            torch.testing.assert_close(out.float(), want.float(), rtol=2 ** -7, atol=2 ** -7)
+
+
 def test_three_operators_in_a_graph(hip):
     """Captured and replayed with eager work between the replays: every replay gives what eager calls give."""
     heads, kv, dim, lens = 8, 2, 64, [700, 130, 65]
@@ -617,6 +716,82 @@ def test_three_operators_in_a_graph(hip):
         graph.replay()
         for a, b in zip([*got, *state], want):
             assert torch.equal(a, b)
+
+
+def test_two_graphs_and_two_streams_at_once(hip):
+    """Workspaces belong to the call: graphs replayed in turn and streams that run at the same time do not meet."""
+    cases = []
+    for n, (q_lens, lens) in enumerate((([1] * 4, [1500, 900, 1100, 40]), ([1, 90], [700, 400]))):
+        ctx, cache = Ctx(q_lens, lens), Cache(lens, 2, 16, 64, torch.bfloat16, seed=10 * n)
+        qkv = rnd(ctx.n_tokens, 8 * 64, dtype=torch.bfloat16, seed=n)
+        start = [t.clone() for t in (cache.k_pages, cache.v_pages, cache.weights)]
+
+        def step(ctx=ctx, cache=cache, qkv=qkv):
+            out = hip.weighed_attention(qkv, 4, 2, 64, 0.125, ctx, cache)
+            return [out, *hip.evict_cache(ctx, cache, 300, keep_first=2, keep_last=50), cache.k_pages, cache.v_pages, cache.weights]
+
+        def reset(cache=cache, start=start):
+            for t, x in zip((cache.k_pages, cache.v_pages, cache.weights), start):
+                t.copy_(x)
+
+        want = [t.clone() for t in step()]
+        reset()
+        cases.append((step, reset, want))
+    graphs = []
+    for step, reset, _ in cases:
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        graphs.append((graph, got))
+        reset()
+    for _ in range(3):
+        for (graph, got), (step, reset, want) in zip(graphs, cases):
+            reset()
+            graph.replay()
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        results = []
+        for stream, (step, reset, _) in zip(streams, cases):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                reset()
+                results.append(step())
+        torch.cuda.synchronize()
+        for got, (_, _, want) in zip(results, cases):
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+
+
+def test_pages_beyond_32_bits(hip):
+    """A pool whose last pages lie more than 2^32 bytes, and 2^31 elements, behind the first."""
+    kv, dim, page = 2, 256, 16
+    n_pages = (1 << 31) // (kv * dim * page) + 40
+    lens, ctx = [300, 77], Ctx([1, 77], [300, 77])
+    cache = Cache(lens, kv, page, dim, torch.bfloat16)
+    small, far = (cache.k_pages, cache.v_pages, cache.block_table), n_pages - cache.k_pages.shape[0]
+    big_k = torch.empty(n_pages, kv, page, dim, dtype=torch.bfloat16, device=DEV)
+    big_v = torch.empty(n_pages, kv, dim, page, dtype=torch.bfloat16, device=DEV)
+    big_k[far:], big_v[far:] = small[0], small[1]
+    cos, sin = angles(300, 128)
+    qkv, weights = rnd(78, 8 * dim, dtype=torch.bfloat16, seed=3), cache.weights.clone()
+    where = ctx.positions[None].contiguous()
+
+    def step(rows):
+        hip.rope_axes_kv_write(rows, 4, kv, dim, (128,), cos, sin, where, ctx, cache)
+        return hip.weighed_attention(rows, 4, kv, dim, 0.0625, ctx, cache), *hip.evict_cache(ctx, cache, 50, keep_last=9), cache.weights
+
+    want = [t.clone() for t in step(qkv.clone())]
+    cache.weights.copy_(weights)
+    k, v = small[0].clone(), small[1].clone()
+    cache.k_pages, cache.v_pages = big_k, big_v
+    cache.block_table = torch.where(small[2] >= 0, small[2] + far, small[2])
+    for a, b in zip(step(qkv.clone()), want):
+        assert torch.equal(a, b)
+    assert torch.equal(big_k[far:], k) and torch.equal(big_v[far:], v)
 
 
 def test_on_a_stream_of_its_own(hip):
