@@ -607,7 +607,7 @@ __global__ __launch_bounds__(PF_WAVES* SIA_WAVE) void attn_prefill_kernel(
         const int row = row0 + n * 16 + r;
         if (row >= q_len) continue;
         const float total = sm.l[n] + sink_term(sinks, head, sm.m[n]), inv = 1.f / total;
-        if (STATS && g == 0) row_stats[(size_t)(q_begin + row) * n_heads + head] = sm.m[n] + log2f(total);
+        if (STATS && g == 0) row_stats[(size_t)(q_begin + row) * n_heads + head] = sm.m[n] + __builtin_amdgcn_logf(total);
         bf16_t* dst = out + ((size_t)(q_begin + row) * n_heads + head) * HD;
 #pragma unroll
         for (int db = 0; db < DBLOCKS; ++db) {
