@@ -29,17 +29,31 @@ __host__ __device__ inline int block_chunks(int q_len, int length, int key0, int
     return tokens > 0 ? (tokens * group + chunk_rows - 1) / chunk_rows : 0;
 }
 
+// Blocks that all of a run's rows see: every one has as many chunks.
+__host__ __device__ inline int full_blocks(int q_len, int length, int keys) { return length >= q_len ? (length - q_len) / keys + 1 : 0; }
+
 // A workgroup's work: a block of keys and rows row_begin .. row_end-1 of a run that begins at token q_begin, place start.
 struct Work {
     int seq, q_begin, q_len, length, start, key0, row_begin, row_end;
 };
 
-// The index-th piece of work of a run; false if there are not so many.  A lane a block: a walk from one to the next would take longer than the work.
+// The index-th piece of work of a run; false if there are not so many.  Behind the blocks that all rows see a lane a block: a walk from one to the next
+// would take longer than the work.
 template <int KEYS>
 __device__ __forceinline__ bool find_work(Work& work, int index, int seq, const int* __restrict__ cu_q, const int* __restrict__ kv_len, int group,
                                           int chunk_rows, int most_keys) {
     const int lane = threadIdx.x % SIA_WAVE, q_begin = cu_q[seq], q_len = cu_q[seq + 1] - q_begin, length = min(kv_len[seq], most_keys);
-    for (int k0 = 0; k0 < length; k0 += SIA_WAVE * KEYS) {
+    const int full = full_blocks(q_len, length, KEYS), each_full = block_chunks(q_len, length, 0, group, chunk_rows);
+    if (each_full <= 0) return false;
+    auto piece = [&](int key0, int chunk, int chunks) {
+        const int tokens = min(q_len, length - key0), rows = tokens * group, first = (q_len - tokens) * group;
+        const int each = ((rows + chunks - 1) / chunks + 31) / 32 * 32;
+        work = Work{seq, q_begin, q_len, length, length - q_len, key0, first + min(chunk * each, rows), first + min((chunk + 1) * each, rows)};
+        return true;
+    };
+    if (index < full * each_full) return piece(index / each_full * KEYS, index % each_full, each_full);
+    index -= full * each_full;
+    for (int k0 = full * KEYS; k0 < length; k0 += SIA_WAVE * KEYS) {
         const int mine = block_chunks(q_len, length, k0 + lane * KEYS, group, chunk_rows);
         int upto = mine;
 #pragma unroll
@@ -52,12 +66,8 @@ __device__ __forceinline__ bool find_work(Work& work, int index, int seq, const 
             index -= __builtin_amdgcn_readlane(upto, SIA_WAVE - 1);
             continue;
         }
-        const int at = __builtin_ctzll(behind), chunks = __builtin_amdgcn_readlane(mine, at), key0 = k0 + at * KEYS;
-        index -= __builtin_amdgcn_readlane(upto, at) - chunks;
-        const int tokens = min(q_len, length - key0), rows = tokens * group, first = (q_len - tokens) * group;
-        const int each = ((rows + chunks - 1) / chunks + 31) / 32 * 32;
-        work = Work{seq, q_begin, q_len, length, length - q_len, key0, first + min(index * each, rows), first + min((index + 1) * each, rows)};
-        return true;
+        const int at = __builtin_ctzll(behind), chunks = __builtin_amdgcn_readlane(mine, at);
+        return piece(k0 + at * KEYS, index - __builtin_amdgcn_readlane(upto, at) + chunks, chunks);
     }
     return false;
 }
@@ -91,10 +101,13 @@ __global__ __launch_bounds__(KEYS) void weigh_add_kernel(const float* __restrict
     const int q_len = cu_q[seq + 1] - cu_q[seq], length = min(kv_len[seq], most_keys), start = length - q_len;
     const int chunks = block_chunks(q_len, length, key0, group, chunk_rows);
     if (chunks <= 0) return;
-    int first = 0;      // the pieces of the blocks before
-    for (int k = (int)(threadIdx.x % SIA_WAVE) * KEYS; k < key0; k += SIA_WAVE * KEYS) first += block_chunks(q_len, length, k, group, chunk_rows);
+    // the pieces of the blocks before
+    const int full = min(full_blocks(q_len, length, KEYS), (int)blockIdx.y);
+    int first = 0;
+    for (int k = (full + (int)(threadIdx.x % SIA_WAVE)) * KEYS; k < key0; k += SIA_WAVE * KEYS) first += block_chunks(q_len, length, k, group, chunk_rows);
 #pragma unroll
     for (int off = SIA_WAVE / 2; off > 0; off >>= 1) first += __shfl_xor(first, off, SIA_WAVE);
+    first += full * block_chunks(q_len, length, 0, group, chunk_rows);
     float* row = weight_row(w, seq, n_kv, hk);
     if (j >= length || !row) return;
     const float old = j < start ? row[j] : 0.f;
@@ -158,8 +171,9 @@ inline Cut cut_runs(int total_tokens, int q_bound, int n_runs, int max_kv, int g
     if (rows > 4096.0) rows = work / fill / 4.0;
     Cut cut;
     cut.chunk_rows = rows < least ? least : rows > 1e9 ? 1 << 30 : ((int)rows + 31) / 32 * 32;
-    cut.most_work = 0;
-    for (long long key0 = 0; key0 < max_kv; key0 += keys) cut.most_work += block_chunks(q_bound, max_kv, (int)key0, group, cut.chunk_rows);
+    const int full = full_blocks(q_bound, max_kv, keys);
+    cut.most_work = full * block_chunks(q_bound, max_kv, 0, group, cut.chunk_rows);
+    for (long long key0 = (long long)full * keys; key0 < max_kv; key0 += keys) cut.most_work += block_chunks(q_bound, max_kv, (int)key0, group, cut.chunk_rows);
     cut.floats = (long long)q_bound * group <= cut.chunk_rows ? 0 : (long long)n_runs * cut.most_work * n_kv * keys;
     return cut;
 }
