@@ -73,9 +73,10 @@ __global__ __launch_bounds__(SELECT_THREADS) void evict_select_kernel(
     const int hk = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid % SIA_WAVE, wave = tid / SIA_WAVE;
     const size_t unit = (size_t)seq * n_kv + hk;
     const int slot = slots[seq], length = max(0, min(kv_len[seq], min(max_kv, places)));
-    if (hk == 0 && tid == 0) lengths[seq] = min(length, budget);
+    const bool none = slot < 0 || slot >= n_slots;      // no row of sums: all stays
+    if (hk == 0 && tid == 0) lengths[seq] = none ? length : min(length, budget);
     int* keep_row = kept + unit * budget;
-    if (length <= budget || slot < 0 || slot >= n_slots) {
+    if (length <= budget || none) {
         for (int i = tid; i < budget; i += SELECT_THREADS) keep_row[i] = i < length ? i : -1;
         if (tid == 0) n_moves[unit] = make_int2(-1, -1);      // nothing moves, the last places neither
         return;

@@ -2118,7 +2118,7 @@ class HipKernels:
         ``cache.weights`` (ties: the lowest place; NaN counts as minus infinity), ``budget`` in all.  Keys, values and weights are
         moved within the sequence's pages, which it must not share: with ``edge = budget - keep_last``, what is kept below the edge stays where it is, the
         kept places from the edge on fill the holes below it, both in order, and the last ``keep_last`` move up together to the edge.  What
-        lies behind the new length stays as it was.  Returns ``(kept, lengths)``: int32 ``[n_seqs, n_kv, budget]``, the
+        lies behind the new length stays as it was; a sequence whose state slot is none keeps all that it has.  Returns ``(kept, lengths)``: int32 ``[n_seqs, n_kv, budget]``, the
         place from which a place's content came (-1 behind the last), and int32 ``[n_seqs]``, the new lengths.  ``ctx`` itself is not changed: the
         next step's places begin at the new lengths (``CacheManager.shrink`` keeps the books)."""
         budget, keep_first, keep_last = int(budget), int(keep_first), int(keep_last)

@@ -515,6 +515,19 @@ def test_evict_cache_with_bad_pages_and_slots(hip):
             assert torch.equal(cache.k_pages[there, 0, i % 16], k[here, 0, j % 16])
 
 
+def test_evict_cache_of_a_sequence_without_a_row(hip):
+    """Its length stays what it was: nothing of it has been dropped."""
+    ctx, cache = Ctx([1, 1, 1], [100, 90, 30], [0, 7, -1]), Cache([100, 90, 30], 2, 16, 32, torch.bfloat16)
+    k, v, w = cache.k_pages.clone(), cache.v_pages.clone(), cache.weights.clone()
+    kept, lengths = hip.evict_cache(ctx, cache, 40, keep_first=1, keep_last=8)
+    assert lengths.tolist() == [40, 90, 30]
+    assert kept[1, 1].tolist() == list(range(40)) and kept[2, 0].tolist() == list(range(30)) + [-1] * 10
+    for s in (1, 2):
+        pages = [p for p in cache.block_table[s].tolist() if p >= 0]
+        assert torch.equal(cache.k_pages[pages], k[pages]) and torch.equal(cache.v_pages[pages], v[pages])
+    assert torch.equal(cache.weights[1:], w[1:])
+
+
 def test_evict_cache_refuses(hip):
     from simple_inference_amd.kernels import KernelError
     ctx, cache = Ctx([1], [40]), Cache([40], 2, 16, 64, torch.bfloat16)
