@@ -41,10 +41,11 @@ struct RopeAxes {
 // The page of a token's place and the offset in it; page -1 where there is nothing to write to.
 template <typename T>
 __device__ __forceinline__ int page_of(const RopeAxes<T>& a, int token, int& off) {
-    const int place = a.positions[token];
-    const int index = place / a.page_size;
+    off = 0;
+    if (a.n_kv == 0) return -1;
+    const int place = a.positions[token], index = place / a.page_size;
     off = place - index * a.page_size;
-    if (a.n_kv == 0 || place < 0 || index >= a.table_width) return -1;
+    if (place < 0 || index >= a.table_width) return -1;
     const int page = a.block_table[(size_t)a.seq_of_token[token] * a.table_width + index];
     return page >= a.n_pages ? -1 : page;
 }

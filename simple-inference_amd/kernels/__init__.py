@@ -2103,7 +2103,7 @@ class HipKernels:
                 run_kv, max_kv, n_heads, n_kv_heads, page, float(scale), _ptr(sinks), weights.data_ptr(), ctx.state_slots.data_ptr(), slots,
                 places, stream), "attn_weighed")
             return out
-        q_bound = max(ctx.q_lens)
+        q_bound = int(ctx.max_q_len)
         ws = weights.new_empty((self.core.sia_attention_weighed_workspace(n, q_bound, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim),))
         self._check(self.core.sia_attention_weighed(
             *given, ctx.seq_of_token.data_ptr(), ctx.positions.data_ptr(), ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), out.data_ptr(),
