@@ -122,7 +122,7 @@ __global__ __launch_bounds__(DEC_WAVES* SIA_WAVE) void attn_decode_kernel(
             ++done;
             run_end = begin(run0 + done + 1);
         }
-        __device__ __forceinline__ void operator()(int kb) {
+        __device__ __forceinline__ void operator()(int kb, Stage&) {
             while (done < mine_n - 1 && kb / TILE >= run_end) pass();  // wave-uniform
         }
     } at_run_ends{0, run_begin(run0 + 1), mine_n, run0, r, g, group, sm, acc, run_begin, row_of};
@@ -312,6 +312,13 @@ __device__ __forceinline__ void tile_fetch(TileRegs<TEAM>& t, const FetchPlan<TE
     }
 }
 
+// A fetched tile's values beyond `last` as zeros (clear_beyond).
+template <int TEAM>
+__device__ __forceinline__ void tile_clear(TileRegs<TEAM>& t, const FetchPlan<TEAM>& plan, int kb, int last) {
+#pragma unroll
+    for (int i = 0; i < TileRegs<TEAM>::PER_THREAD; ++i) clear_beyond(t.v[i], kb + plan.v_key[i], last);
+}
+
 // Writes a fetched tile into an LDS stage.  Key rows are stored in the order the score MFMAs read them
 // (row 16h + m holds key 8(m/4) + 4h + m%4), so that the 16 lanes of a read take 16 consecutive rows.
 template <int TEAM>
@@ -388,7 +395,7 @@ __device__ __forceinline__ void compute_from_lds(const bf16_t* __restrict__ k_ld
 // every KSPLIT-th tile of keys: ROWS = PF_NQ * 16 * PF_WAVES / KSPLIT tokens per workgroup.  KTILES tiles of keys
 // are staged per step (and barrier); with KSPLIT = 1 every wave takes them one after the other, which at 8 waves
 // of 16 tokens is 7 % faster with two tiles than with one (fewer barriers a key) and changes no bit.
-// STATS: leaves every row's m + log2(l) in row_stats (float [token][query head]).
+// STATS: leaves every row's m + log2(l) in row_stats (float [token][query head]), and pages may hold anything behind a sequence's places.
 template <int PF_NQ, int PF_WAVES, int KSPLIT, int KTILES, bool STATS>
 __global__ __launch_bounds__(PF_WAVES* SIA_WAVE) void attn_prefill_kernel(
     const bf16_t* __restrict__ q, int q_row_stride, const bf16_t* __restrict__ kp, const bf16_t* __restrict__ vp,
@@ -509,7 +516,10 @@ __global__ __launch_bounds__(PF_WAVES* SIA_WAVE) void attn_prefill_kernel(
         tile_fetch(SET[p], plan, kp, vp, found[p], ps_log2, page_stride, min((KB) + p * TILE, w_last), blk_lo, blk_hi)
 #define PF_STORE(SET, KB, STAGE)                                                                                \
     _Pragma("unroll") for (int p = 0; p < KTILES; ++p)                                                          \
-        if ((KB) + p * TILE <= w_last) tile_store(SET[p], PF_K_LDS(STAGE, p), PF_V_LDS(STAGE, p), ps_log2)
+        if ((KB) + p * TILE <= w_last) {                                                                        \
+            if (STATS && (KB) + p * TILE + TILE - 1 > blk_hi) tile_clear(SET[p], plan, (KB) + p * TILE, blk_hi); \
+            tile_store(SET[p], PF_K_LDS(STAGE, p), PF_V_LDS(STAGE, p), ps_log2);                                \
+        }
 #define PF_LIVE(MY_KB)                                                                                          \
     (wave_live && (MY_KB) <= w_last && (MY_KB) <= wave_hi &&                                                    \
      ((MY_KB) + TILE - 1 >= wave_lo || (FORMS && (MY_KB) < forms.keep_first)))
@@ -561,8 +571,14 @@ __global__ __launch_bounds__(PF_WAVES* SIA_WAVE) void attn_prefill_kernel(
         if (wave_live) {
             const int range_hi = first_pos + row_last;
             const int range_lo = walk_begin(oldest_of(first_pos + row0), forms.keep_first);
-            attend_range<PF_NQ>(qf, kp, vp, table, table_width, ps_log2, n_kv, hk, range_lo, range_hi, lo, hi, scale,
-                                sm, acc, forms, places);
+            if constexpr (STATS) {
+                ClearBeyond clear{range_hi, g};
+                attend_range<PF_NQ>(qf, kp, vp, table, table_width, ps_log2, n_kv, hk, range_lo, range_hi, lo, hi, scale,
+                                    sm, acc, clear, forms, places);
+            } else {
+                attend_range<PF_NQ>(qf, kp, vp, table, table_width, ps_log2, n_kv, hk, range_lo, range_hi, lo, hi, scale,
+                                    sm, acc, forms, places);
+            }
         }
     }
     sm.finish_sums();

@@ -287,13 +287,37 @@ __device__ __forceinline__ void compute_stage(const Stage& st, const bf16x8 (&q)
             acc[n][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(st.v[db], p[n], acc[n][db], 0, 0, 0);
 }
 
+// Of the 8 values of positions first .. first + 7, those beyond `last` as zeros: pages may hold anything there, and a weight of 0 times a number
+// without bounds is none.
+template <typename Words>      // four 32-bit words
+__device__ __forceinline__ void clear_beyond(Words& u, int first, int last) {
+    const int n = min(max(last - first + 1, 0), 8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] &= n >= 2 * i + 2 ? 0xffffffffu : n == 2 * i + 1 ? 0x0000ffffu : 0u;
+}
+__device__ __forceinline__ void clear_values(Stage& st, int kb, int g, int last) {
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int db = 0; db < DBLOCKS; ++db) {
+        words u = __builtin_bit_cast(words, st.v[db]);
+        clear_beyond(u, kb + 8 * g, last);
+        st.v[db] = __builtin_bit_cast(bf16x8, u);
+    }
+}
+
 // Called before a tile is computed; the default does nothing.
 struct NoHook {
-    __device__ __forceinline__ void operator()(int) const {}
+    __device__ __forceinline__ void operator()(int, Stage&) const {}
+};
+struct ClearBeyond {      // values beyond `last` as zeros
+    int last, g;
+    __device__ __forceinline__ void operator()(int kb, Stage& st) const {
+        if (kb + TILE - 1 > last) clear_values(st, kb, g, last);
+    }
 };
 
 // The tiles w_first, w_first + TILE, ..., w_last, whose block-table entries the window holds; two register
-// stages in turn: the loads of tile t+1 are issued before the arithmetic of tile t.  `before(kb)` runs before the
+// stages in turn: the loads of tile t+1 are issued before the arithmetic of tile t.  `before(kb, stage)` runs before the
 // arithmetic of the tile at kb (it may hand the state on and start it afresh).
 template <int NQ, typename Hook>
 __device__ __forceinline__ void attend_tiles(const PageWindow& pages, int w_first, int w_last,
@@ -307,12 +331,12 @@ __device__ __forceinline__ void attend_tiles(const PageWindow& pages, int w_firs
     for (int kb = w_first; kb <= w_last; kb += 2 * TILE) {
         const int kb1 = min(kb + TILE, w_last);  // past the end: the last tile again, never computed
         load_stage(b, kp, vp, pages, ps_log2, n_kv, hk, kb1, range_lo, range_hi);
-        before(kb);
+        before(kb, a);
         compute_stage<NQ>(a, q, kb, lo, hi, scale, sm, acc, forms);
         const int kb2 = min(kb + 2 * TILE, w_last);
         load_stage(a, kp, vp, pages, ps_log2, n_kv, hk, kb2, range_lo, range_hi);
         if (kb + TILE <= w_last) {
-            before(kb + TILE);
+            before(kb + TILE, b);
             compute_stage<NQ>(b, q, kb + TILE, lo, hi, scale, sm, acc, forms);
         }
     }

@@ -42,20 +42,6 @@ __device__ __forceinline__ void leave_scores(float* __restrict__ mine, int kb, i
     to[1] = make_float4(s[1][0] * scale, s[1][1] * scale, s[1][2] * scale, s[1][3] * scale);
 }
 
-// Values of positions beyond `last` as zeros: pages may hold anything there, and a weight of 0 times a number without bounds is none.
-__device__ __forceinline__ void clear_values(Stage& st, int kb, int g, int last) {
-    const int n = min(max(last - (kb + 8 * g) + 1, 0), 8);      // of this lane's 8 positions
-    uint32_t keep[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) keep[i] = n >= 2 * i + 2 ? 0xffffffffu : n == 2 * i + 1 ? 0x0000ffffu : 0u;
-#pragma unroll
-    for (int db = 0; db < DBLOCKS; ++db) {
-        uint4 u = __builtin_bit_cast(uint4, st.v[db]);
-        u.x &= keep[0], u.y &= keep[1], u.z &= keep[2], u.w &= keep[3];
-        st.v[db] = __builtin_bit_cast(bf16x8, u);
-    }
-}
-
 // grid (groups of query heads, sequences, splits), four waves of a run of tiles each, as attn_decode_kernel's plain mode.  The memory bounds it:  8 rows over
 // 2,048 keys, 24 heads of 128 on 8, 15.1 us and 3.9 for the join (67 MB: 4.4 TB/s), 3 of 32 over 12,000 37.6 and 5.4 (150 MB: 4.0 TB/s).  With the keys and
 // values in the last-level cache a whole call takes 19.1 and 31.3 us, attention alone 18.7 and 29.7.

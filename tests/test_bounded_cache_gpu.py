@@ -377,6 +377,23 @@ def test_weighed_attention_beside_what_it_must_not_read(hip, dtype):
     assert torch.equal(torch.nan_to_num(cache.weights, 7.0), torch.nan_to_num(before, 7.0))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q_lens,kv_lens,heads,kv,dim,page", [
+    ([1, 45], [33, 45], 4, 2, 64, 16), ([1, 1, 300], [31, 700, 1001], 6, 2, 128, 32), ([2100], [2100], 2, 1, 128, 64), ([700, 3, 30], [700, 2603, 61], 8, 2, 80, 8),
+    ([17, 65], [17, 333], 4, 1, 256, 16), ([9, 520], [9, 521], 2, 2, 16, 128), ([40, 33], [75, 33], 4, 2, 100, 16), ([1, 6], [7, 9], 2, 2, 48, 4)])
+def test_weighed_attention_whatever_lies_behind_the_places(hip, dtype, q_lens, kv_lens, heads, kv, dim, page):
+    """Keys and values behind every sequence's places, and pages that are nobody's, without bounds or no numbers."""
+    ctx, cache = Ctx(q_lens, kv_lens), Cache(kv_lens, kv, page, dim, dtype, room=page)
+    spare = torch.ones(cache.k_pages.shape[0], page, dtype=torch.bool, device=DEV)
+    for s, length in enumerate(kv_lens):
+        at = torch.arange(length, device=DEV)
+        spare[cache.block_table[s].long()[at // page], at % page] = False
+    odd = torch.where(rnd(*spare.shape, seed=6) < 0, math.nan, math.inf).to(dtype)
+    cache.k_pages.copy_(torch.where(spare[:, None, :, None], odd[:, None, :, None], cache.k_pages))
+    cache.v_pages.copy_(torch.where(spare[:, None, None, :], odd[:, None, None, :], cache.v_pages))
+    check_weighed(hip, ctx, cache, rnd(ctx.n_tokens, heads * dim, dtype=dtype, seed=8), heads, dim ** -0.5)
+
+
 def test_weighed_attention_refuses(hip):
     from simple_inference_amd.kernels import KernelError
     ctx, cache = Ctx([1, 4], [40, 20]), Cache([40, 20], 2, 16, 64, torch.bfloat16)
