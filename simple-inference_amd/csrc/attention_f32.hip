@@ -250,9 +250,10 @@ __global__ __launch_bounds__(WAVES * SIA_WAVE) void attention_f32_kernel(
         begin = end;
     }
     if (r >= n_rows) return;
+    const bool nothing = row_stats && saw_nothing(m, l);      // (a sequence without places)
     if (sinks) l += expf(sinks[head] - m);
-    if (row_stats && wave == 0 && g == 0) row_stats[(size_t)token * n_heads + head] = row_stat(m, l);
-    const float inv = 1.f / l;
+    if (row_stats && wave == 0 && g == 0) row_stats[(size_t)token * n_heads + head] = nothing ? INFINITY : row_stat(m, l);
+    const float inv = nothing ? 0.f : 1.f / l;
     float* o = out + ((size_t)token * n_heads + head) * value_dim;
 #pragma unroll
     for (int a = 0; a < BLOCKS; ++a) {

@@ -93,9 +93,10 @@ __global__ __launch_bounds__(SIA_WAVE) void attention_generic_kernel(
     }
 
     T* o = out + ((size_t)n * n_heads + h) * value_dim;
+    const bool nothing = row_stats && saw_nothing(m, l);      // (a sequence without places)
     if (sinks) l += expf(sinks[h] - m);   // m is finite: a token always sees itself
-    if (row_stats && lane == 0) row_stats[(size_t)n * n_heads + h] = row_stat(m, l);
-    const float inv = 1.f / l;
+    if (row_stats && lane == 0) row_stats[(size_t)n * n_heads + h] = nothing ? INFINITY : row_stat(m, l);
+    const float inv = nothing ? 0.f : 1.f / l;
 #pragma unroll
     for (int dd = 0; dd < ATTN_MAX_HEAD_DIM / SIA_WAVE; ++dd) {
         const int d = lane + dd * SIA_WAVE;

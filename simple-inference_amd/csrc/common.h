@@ -76,10 +76,11 @@ __device__ __forceinline__ void rotate_pair(float a, float b, float c, float s, 
 }
 
 // What a softmax row leaves for whoever wants its weights afterwards: m + log(l) in units of log2, for a maximum (or any reference) m in
-// natural units and the sum l of exp(s - m).  A row that saw nothing: infinity, so that every weight is 0.
-__device__ __forceinline__ float row_stat(float m, float l) {
-    return l == 0.f ? INFINITY : fmaf(m, 1.4426950408889634f, log2f(l));
-}
+// natural units and the sum l of exp(s - m).
+__device__ __forceinline__ float row_stat(float m, float l) { return fmaf(m, 1.4426950408889634f, log2f(l)); }
+// Whether a row with this maximum and this sum (without a sink's term) saw no key: its result is zeros, and its statistic infinity, so that every
+// weight is 0.
+__device__ __forceinline__ bool saw_nothing(float m, float l) { return m == -INFINITY && l == 0.f; }
 
 // Eight consecutive elements of a row as one register value: 32 bytes of float or 16 of bfloat16.
 template <typename T> struct Vec8;

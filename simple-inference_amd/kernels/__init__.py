@@ -2067,7 +2067,8 @@ class HipKernels:
         ``cache.weights[slot, g, place]`` (float32 ``[slots, n_kv_heads, places]``; a sequence's row is ``ctx.state_slots[s]``, each
         sequence with a row of its own) grows by the sum, over the sequence's tokens of this step and the query heads of ``g``, of
         their softmax weights.  The sums of the places that the step itself has written begin at zero.  ``sinks`` take their share
-        of a row's weight and have no place.  Prompts, portions and single tokens, mixed as ``ctx`` says."""
+        of a row's weight and have no place.  A row of a sequence without places is zeros.  Prompts, portions and single tokens, mixed as
+        ``ctx`` says."""
         self._want(qkv, "qkv")
         if qkv.dtype not in _DT or qkv.dim() != 2:
             raise KernelError(f"qkv must be a float32 or bfloat16 matrix, is {qkv.dtype} {tuple(qkv.shape)}")
