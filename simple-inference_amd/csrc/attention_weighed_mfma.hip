@@ -282,20 +282,25 @@ __device__ __forceinline__ void weigh_rows(floatx4 (&sum)[WAVE_BLOCKS], const bf
         }
     }
     const bool whole = __builtin_amdgcn_readfirstlane(place[0]) >= k0 + WAVE_KEYS - 1;
-    if (!whole) {
+    if (whole) {
 #pragma unroll
         for (int h = 0; h < HALVES; ++h)
 #pragma unroll
             for (int v = 0; v < WAVE_BLOCKS; ++v)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[h][v][i] = k0 + v * 16 + g * 4 + i <= place[h] ? s[h][v][i] : -INFINITY;
+                for (int i = 0; i < 4; ++i) sum[v][i] += fast_exp2(fmaf(s[h][v][i], scale, -stat[h]));
+        return;
     }
+    // A key that a row does not see gets nothing of it, whatever the row's scores and statistic are.
 #pragma unroll
     for (int h = 0; h < HALVES; ++h)
 #pragma unroll
         for (int v = 0; v < WAVE_BLOCKS; ++v)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum[v][i] += fast_exp2(fmaf(s[h][v][i], scale, -stat[h]));
+            for (int i = 0; i < 4; ++i) {
+                const float p = fast_exp2(fmaf(s[h][v][i], scale, -stat[h]));
+                sum[v][i] += k0 + v * 16 + g * 4 + i <= place[h] ? p : 0.f;
+            }
 }
 
 __global__ __launch_bounds__(RUN_THREADS) void weigh_runs_kernel(

@@ -29,3 +29,25 @@ def test_sequences_without_places(hip, dtype, sinks, dim, vdim, page):
     out = check_weighed(hip, ctx, cache, qkv, 4, dim ** -0.5, sinks=sinks, poison=False)
     assert torch.equal(out[[0, 2]], torch.zeros_like(out[[0, 2]]))
     assert torch.equal(cache.weights[[2, 5, 3, 4]], before[[2, 5, 3, 4]])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q,length,heads,kv,dim,page", [(50, 50, 4, 2, 64, 16), (300, 420, 6, 2, 128, 16), (90, 400, 2, 1, 256, 32), (65, 65, 4, 2, 22, 12),
+                                                        (600, 601, 8, 1, 80, 8)])
+def test_a_row_that_is_no_number_spoils_only_what_it_sees(hip, dtype, q, length, heads, kv, dim, page):
+    """One token's query of the first head is NaN: the sums of the first group's keys up to that token's place are, those beyond are not."""
+    ctx, cache = Ctx([q], [length]), Cache([length], kv, page, dim, dtype)
+    qkv, at, start = rnd(q, heads * dim, dtype=dtype, seed=8), q // 3, length - q
+    other, before = qkv.clone(), cache.weights.clone()
+    qkv[at, :dim] = math.nan
+    other[at, :dim] = 0
+    scale = dim ** -0.5
+    out = hip.weighed_attention(qkv, heads, kv, dim, scale, ctx, cache)
+    got = cache.weights.clone()
+    assert out[at, :dim].isnan().all()
+    assert got[0, 0, :start + at + 1].isnan().all()
+    cache.weights.copy_(before)
+    want = check_weighed(hip, ctx, cache, other, heads, scale, poison=False)      # a query of zeros weighs no key beyond its place either
+    out[at, :dim] = want[at, :dim]
+    assert torch.equal(out, want)
+    assert torch.equal(got[0, 0, start + at + 1:], cache.weights[0, 0, start + at + 1:]) and torch.equal(got[0, 1:], cache.weights[0, 1:])
