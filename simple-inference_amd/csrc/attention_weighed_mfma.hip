@@ -445,9 +445,9 @@ SIA_EXPORT long long sia_attn_weighed_workspace(int n_single, int n_seqs, int n_
     return floats;
 }
 
-// Sequences 0 .. n_single-1 of the step bring one token each, which is row s of q, and none is longer than max_kv; sequences n_single .. n_seqs-1
-// bring at most q_bound tokens over at most run_kv places, n_tokens - n_single in all, in row tiles as sia_attn_prefill counts them.  weights
-// [n_slots][n_kv][places], a sequence's row at slots[s].
+// Sequences 0 .. n_single-1 of the step bring one token each, which is row s of q, and none of them is longer than max_kv (without such: no sequence
+// is); sequences n_single .. n_seqs-1 bring at most q_bound tokens over at most run_kv places, n_tokens - n_single in all, in row tiles as
+// sia_attn_prefill counts them.  weights [n_slots][n_kv][places], a sequence's row at slots[s].
 SIA_EXPORT int sia_attn_weighed(const void* q, int q_row_stride, const void* k_pages, const void* v_pages, const int* block_table, int table_width,
                                 const int* cu_q, const int* kv_len, void* out, float* ws, int n_single, int n_seqs, int n_tokens, int n_tiles,
                                 int n_tiles_split, int n_tiles_long, int q_bound, int run_kv, int max_kv, int n_heads, int n_kv, int page_size,
@@ -457,7 +457,7 @@ SIA_EXPORT int sia_attn_weighed(const void* q, int q_row_stride, const void* k_p
     const bool runs = n_runs > 0 && q_bound > 0 && n_tokens > n_single;
     if (ps_log2 < 3 || n_kv <= 0 || n_heads % n_kv || n_heads / n_kv > JOIN_MOST_HEADS || n_heads > 65535 || n_seqs > 65535 || n_single < 0 || n_runs < 0 ||
         q_row_stride % 8 || table_width <= 0 || max_kv <= 0 || places < max_kv || n_slots <= 0 || !ws || !weights || !(scale > 0.f) ||
-        (runs && (run_kv <= 0 || run_kv > max_kv || (long long)q_bound * (n_heads / n_kv) > 0x7fffff00)))
+        (runs && (run_kv <= 0 || run_kv > (n_single > 0 ? places : max_kv) || (long long)q_bound * (n_heads / n_kv) > 0x7fffff00)))
         return SIA_BAD_ARGUMENT;
     const Cut cut = runs ? cut_of(n_tokens - n_single, q_bound, n_runs, run_kv, n_heads, n_kv) : Cut{};
     if (runs && (cut.most_work > 65535 || (run_kv + RUN_KEYS - 1) / RUN_KEYS > 65535)) return SIA_BAD_ARGUMENT;

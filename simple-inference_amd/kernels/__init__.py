@@ -508,7 +508,7 @@ class HipKernels:
                                              _ptr(positions), _ptr(kv_len), _ptr(seq), _ptr(cu_q), _ptr(own), n, self._stream()),
                     "rows_alone")
         alone = dataclasses.replace(ctx, n_tokens=n, n_seqs=n, positions=positions, seq_of_token=seq, cu_q=cu_q, kv_len=kv_len,
-                                    max_q_len=1, n_decode_seqs=n, q_lens=[1] * n, max_run_kv_len=0, only_rows=None)
+                                    max_q_len=1, n_decode_seqs=n, q_lens=[1] * n, max_run_kv_len=0, max_single_kv_len=0, only_rows=None)
         return alone, dataclasses.replace(cache, block_table=own)
 
     def embed(self, token_ids, table, scale=1.0):
@@ -2098,6 +2098,8 @@ class HipKernels:
             # single tokens by one walk over keys and values, runs by the attention kernel and the scores once more
             lib = self._attn_lib(head_dim)
             tiles, q_bound, run_kv = self._run_tiles(lib, ctx) if n_single < ctx.n_seqs else ((0, 0, 0), 0, 0)
+            if n_single:      # scores, splits and the join's grid are those of the longest single token
+                max_kv = self._single_kv(ctx, max_kv)
             ws = weights.new_empty((lib.sia_attn_weighed_workspace(n_single, ctx.n_seqs, n, q_bound, run_kv, max_kv, n_heads, n_kv_heads),))
             self._check(lib.sia_attn_weighed(
                 *given, ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), out.data_ptr(), ws.data_ptr(), n_single, ctx.n_seqs, n, *tiles, q_bound,
@@ -2144,6 +2146,11 @@ class HipKernels:
             budget, keep_first, keep_last, kept.data_ptr(), lengths.data_ptr(), ws.data_ptr(), _DT[k_pages.dtype], self._stream_here()),
             "evict")
         return kept, lengths
+
+    @staticmethod
+    def _single_kv(ctx, max_kv):
+        """What bounds the keys of the step's single tokens; ``max_kv``: those of all its sequences."""
+        return max_kv if ctx.kv_bound else min(max_kv, int(getattr(ctx, "max_single_kv_len", 0) or max_kv))
 
     @staticmethod
     def _run_tiles(lib, ctx):

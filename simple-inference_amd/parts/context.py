@@ -48,6 +48,7 @@ class StepContext:
     q_lens: list = field(default_factory=list)  # host copy: tokens each sequence brings
     kv_bound: int = 0  # replayed graphs: an upper bound of kv_len that fixes grids (0: use max_kv_len)
     max_run_kv_len: int = 0  # the longest kv_len among the sequences that bring more than one token (0: not known)
+    max_single_kv_len: int = 0  # the longest among those that bring one (0: not known)
     extra: dict = field(default_factory=dict)  # name -> int32 [n_tokens]: what the step's entries brought beside tokens
     shared: dict = field(default_factory=dict)  # name -> what a layer of this step leaves for later layers of the step
     only_rows: Optional[torch.Tensor] = None  # set for a mixer that ``gives_only_rows``: the only rows of its result that are read

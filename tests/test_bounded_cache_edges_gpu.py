@@ -51,3 +51,31 @@ def test_a_row_that_is_no_number_spoils_only_what_it_sees(hip, dtype, q, length,
     out[at, :dim] = want[at, :dim]
     assert torch.equal(out, want)
     assert torch.equal(got[0, 0, start + at + 1:], cache.weights[0, 0, start + at + 1:]) and torch.equal(got[0, 1:], cache.weights[0, 1:])
+
+
+def grown_by(call):
+    """Bytes of GPU memory that a call has at most beside what there was before it."""
+    call()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    there = torch.cuda.memory_allocated()
+    call()
+    return torch.cuda.max_memory_allocated() - there
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16])
+def test_short_rows_beside_a_long_run(hip, dtype):
+    """Single tokens over some tens of keys, one of them over nothing but itself, beside a portion over thousands: right, and with workspaces for
+    the keys and rows that there are."""
+    q_lens, lens, heads, kv, dim = [1] * 40 + [300], [1 + 7 * i % 60 for i in range(40)] + [5000], 8, 2, 64
+    ctx, cache = Ctx(q_lens, lens), Cache(lens, kv, 16, dim, dtype)
+    ctx.max_single_kv_len = max(lens[:40])
+    qkv = rnd(ctx.n_tokens, heads * dim, dtype=dtype, seed=8)
+    check_weighed(hip, ctx, cache, qkv, heads, 0.125)
+    # results, statistics, scores of 40 rows over at most 64 keys with their states, and pieces of the run's rows over its keys: some 4 (8 in
+    # float32) of 64 query rows for each of 5,000 keys and 2 heads
+    rows = qkv.numel() * qkv.element_size() + ctx.n_tokens * heads * 4 + 40 * heads * (64 + 66) * 4
+    assert grown_by(lambda: hip.weighed_attention(qkv, heads, kv, dim, 0.125, ctx, cache)) < 2 * rows + 20 * 5200 * kv * 4
+    out = hip.weighed_attention(qkv, heads, kv, dim, 0.125, ctx, cache)
+    ctx.max_single_kv_len = 0                    # not known: the step's own bound
+    assert torch.equal(hip.weighed_attention(qkv, heads, kv, dim, 0.125, ctx, cache), out)
