@@ -79,16 +79,23 @@ __device__ __forceinline__ f32x4 load4(const bf16_t* p) {
 
 // What bounds it at a few hundred tokens is the chain of loads before the first product; then the float products (157 TFLOP/s).  Three tokens over 200
 // and a prompt of 300, 32 heads of 64 on 8: 13 us beside an attention of 18.3 and a sum of the chunks of 2.6 to 3.9; the plain kernel 7,400.
-// DP: 32, 64, 128 or 256, the head sizes' upper bound.  grid and parts as weigh_runs_kernel's.
+// DP: 32, 64, 128 or 256, the head sizes' upper bound.  The items of a key/value head are blocks keys' blocks of each of the first n_direct sequences,
+// which bring one token each (one chunk a block: straight into the weights), then most_work pieces of work of each of the others, which have parts as
+// weigh_runs_kernel's.  grid (key/value heads, items in rows of gridDim.y).
 template <typename T, int DP>
 __global__ __launch_bounds__(F32_WAVES* SIA_WAVE) void weigh_float_kernel(
     const T* __restrict__ q, int q_row_stride, const T* __restrict__ k_pages, const int* __restrict__ block_table, int table_width,
     const int* __restrict__ cu_q, const int* __restrict__ kv_len, const float* __restrict__ row_stats, int n_heads, int n_kv, int head_dim,
-    int page_size, int n_pages, float scale, int chunk_rows, int most_keys, float* __restrict__ parts, const Weighed w) {
+    int page_size, int n_pages, float scale, int chunk_rows, int most_keys, int n_direct, int blocks, int most_work, int items,
+    float* __restrict__ parts, const Weighed w) {
     constexpr int PIECES = DP / 16, F32_BLOCKS = f32_blocks(DP), F32_WAVE_KEYS = 16 * F32_BLOCKS, F32_KEYS = f32_keys(DP);
     const int hk = blockIdx.x, group = n_heads / n_kv;
+    const unsigned item = blockIdx.z * gridDim.y + blockIdx.y;
+    if (item >= (unsigned)items) return;
+    const int piece = (int)item - n_direct * blocks;      // of the others', if not negative
+    const unsigned each = piece < 0 ? blocks : most_work, at = piece < 0 ? item : (unsigned)piece, nth = at / each;
     Work run;
-    if (!find_work<F32_KEYS>(run, blockIdx.y, blockIdx.z, cu_q, kv_len, group, chunk_rows, most_keys)) return;
+    if (!find_work<F32_KEYS>(run, (int)(at - nth * each), (int)nth + (piece < 0 ? 0 : n_direct), cu_q, kv_len, group, chunk_rows, most_keys)) return;
     const int wave = threadIdx.x / SIA_WAVE, lane = threadIdx.x % SIA_WAVE, r = lane & 15, g = lane >> 4;
     const int k0 = run.key0 + wave * F32_WAVE_KEYS;
     if (k0 >= run.length) return;
@@ -162,7 +169,7 @@ __global__ __launch_bounds__(F32_WAVES* SIA_WAVE) void weigh_float_kernel(
         fetch(qa, sa, pa);
         compute(qb, sb, pb);
     }
-    leave_sums(sum, k0, run, parts ? parts + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * n_kv + hk) * F32_KEYS : nullptr, w, n_kv, hk);
+    leave_sums(sum, k0, run, parts && piece >= 0 ? parts + ((size_t)piece * n_kv + hk) * F32_KEYS : nullptr, w, n_kv, hk);
 }
 
 // Whether weigh_float_kernel takes such heads and rows.
@@ -171,22 +178,26 @@ static bool float_takes(const void* q, int q_row_stride, const void* k_pages, in
 }
 
 // How the sequences of a launch are cut: three workgroups are on a compute unit at a time.
+constexpr int F32_LEAST_ROWS = 64;
 static Cut cut_float(int n_tokens, int q_bound, int n_seqs, int max_kv, int n_heads, int n_kv, int head_dim) {
-    return cut_runs(n_tokens, q_bound, n_seqs, max_kv, n_heads / n_kv, n_kv, f32_keys(head_dim), 64, 768);
+    return cut_runs(n_tokens, q_bound, n_seqs, max_kv, n_heads / n_kv, n_kv, f32_keys(head_dim), F32_LEAST_ROWS, 768);
 }
+// Of n_single sequences of a token each, those whose rows fill no chunk: all or none.  They need no parts.
+static int direct_of(int n_single, int group) { return group <= F32_LEAST_ROWS ? n_single : 0; }
 
 template <typename T, int DP>
 static int weigh_float(const T* q, int q_row_stride, const T* k_pages, const int* block_table, int table_width, const int* cu_q, const int* kv_len,
-                       const float* row_stats, float* parts, int n_seqs, int max_kv, int n_heads, int n_kv, int head_dim, int page_size, int n_pages,
-                       float scale, const Cut& cut, const Weighed& w, hipStream_t stream) {
+                       const float* row_stats, float* parts, int n_direct, int n_seqs, int max_kv, int n_heads, int n_kv, int head_dim, int page_size,
+                       int n_pages, float scale, const Cut& cut, const Weighed& w, hipStream_t stream) {
     const int most_keys = (int)min((long long)max_kv, (long long)table_width * page_size), blocks = (max_kv + f32_keys(DP) - 1) / f32_keys(DP);
-    if (cut.most_work > 65535 || blocks > 65535) return SIA_BAD_ARGUMENT;
-    hipLaunchKernelGGL((weigh_float_kernel<T, DP>), dim3(n_kv, cut.most_work, n_seqs), dim3(F32_WAVES * SIA_WAVE), 0, stream, q, q_row_stride, k_pages,
-                       block_table, table_width, cu_q, kv_len, row_stats, n_heads, n_kv, head_dim, page_size, n_pages, scale, cut.chunk_rows,
-                       most_keys, parts, w);
+    const long long items = (long long)n_direct * blocks + (long long)(n_seqs - n_direct) * cut.most_work, rows = (items + 65534) / 65535;
+    if (blocks > 65535 || items > 0x7fff0000) return SIA_BAD_ARGUMENT;
+    hipLaunchKernelGGL((weigh_float_kernel<T, DP>), dim3(n_kv, (unsigned)((items + rows - 1) / rows), (unsigned)rows), dim3(F32_WAVES * SIA_WAVE), 0,
+                       stream, q, q_row_stride, k_pages, block_table, table_width, cu_q, kv_len, row_stats, n_heads, n_kv, head_dim, page_size, n_pages,
+                       scale, cut.chunk_rows, most_keys, n_direct, blocks, cut.most_work, (int)items, parts, w);
     if (parts)
-        hipLaunchKernelGGL(weigh_add_kernel<f32_keys(DP)>, dim3(n_kv, blocks, n_seqs), dim3(f32_keys(DP)), 0, stream, parts, cu_q, kv_len, n_heads,
-                           n_kv, 0, cut.chunk_rows, most_keys, cut.most_work, w);
+        hipLaunchKernelGGL(weigh_add_kernel<f32_keys(DP)>, dim3(n_kv, blocks, n_seqs - n_direct), dim3(f32_keys(DP)), 0, stream, parts, cu_q, kv_len,
+                           n_heads, n_kv, n_direct, cut.chunk_rows, most_keys, cut.most_work, w);
     return SIA_LAUNCH_CHECK();
 }
 
@@ -199,9 +210,12 @@ extern "C" int sia_attention_generic_stats(const void*, int, const void*, const 
                                            int, int, int, float, const float*, float*, int, hipStream_t);
 
 // Floats that sia_attention_weighed's workspace holds (arguments as there).
-SIA_EXPORT long long sia_attention_weighed_workspace(int n_tokens, int q_bound, int n_seqs, int max_kv, int n_heads, int n_kv, int head_dim) {
-    if (n_tokens <= 0 || q_bound <= 0 || n_seqs <= 0 || max_kv <= 0 || n_heads <= 0 || n_kv <= 0 || n_heads % n_kv) return 0;
-    return (long long)n_tokens * n_heads + cut_float(n_tokens, q_bound, n_seqs, max_kv, n_heads, n_kv, head_dim).floats;
+SIA_EXPORT long long sia_attention_weighed_workspace(int n_tokens, int n_single, int q_bound, int n_seqs, int max_kv, int n_heads, int n_kv,
+                                                     int head_dim) {
+    if (n_tokens <= 0 || q_bound <= 0 || n_seqs <= 0 || n_single < 0 || n_single > n_seqs || max_kv <= 0 || n_heads <= 0 || n_kv <= 0 || n_heads % n_kv)
+        return 0;
+    const int n_cut = n_seqs - direct_of(n_single, n_heads / n_kv);
+    return (long long)n_tokens * n_heads + cut_float(n_tokens, q_bound, n_cut, max_kv, n_heads, n_kv, head_dim).floats;
 }
 
 // The arguments of the attention kernels without window, blocks and forms; q: rows of the step's tokens; n_single: that many sequences, the first
@@ -215,7 +229,7 @@ SIA_EXPORT int sia_attention_weighed(const void* q, int q_row_stride, const void
     if (n_tokens <= 0 || n_seqs <= 0) return 0;
     if ((dtype != SIA_F32 && dtype != SIA_BF16) || head_dim <= 0 || head_dim > WEIGH_MAX_HEAD_DIM || value_dim <= 0 || n_heads <= 0 || n_kv <= 0 || n_heads % n_kv ||
         n_heads > 65535 || n_seqs > 65535 || page_size <= 0 || table_width <= 0 || n_pages <= 0 || q_bound <= 0 || max_kv <= 0 || places < max_kv ||
-        n_slots <= 0 || !ws || !weights || (long long)q_bound * (n_heads / n_kv) > 0x7fffff00)
+        n_slots <= 0 || !ws || !weights || n_single < 0 || n_single > n_seqs || (long long)q_bound * (n_heads / n_kv) > 0x7fffff00)
         return SIA_BAD_ARGUMENT;
     float* stats = ws;
     int rc = dtype == SIA_F32 ? sia_attention_f32_stats((const float*)q, q_row_stride, (const float*)k_pages, (const float*)v_pages, block_table, table_width,
@@ -232,11 +246,12 @@ SIA_EXPORT int sia_attention_weighed(const void* q, int q_row_stride, const void
         return weigh_plain((const bf16_t*)q, q_row_stride, (const bf16_t*)k_pages, block_table, table_width, cu_q, kv_len, stats, n_seqs, max_kv, n_heads, n_kv,
                            head_dim, page_size, n_pages, scale, w, stream);
     }
-    const Cut cut = cut_float(n_tokens, q_bound, n_seqs, max_kv, n_heads, n_kv, head_dim);
+    const int n_direct = direct_of(n_single, n_heads / n_kv);
+    const Cut cut = cut_float(n_tokens, q_bound, n_seqs - n_direct, max_kv, n_heads, n_kv, head_dim);
     float* parts = cut.floats ? stats + (long long)n_tokens * n_heads : nullptr;
 #define OF_SIZE(T, DP)                                                                                                                                  \
-    weigh_float<T, DP>((const T*)q, q_row_stride, (const T*)k_pages, block_table, table_width, cu_q, kv_len, stats, parts, n_seqs, max_kv, n_heads, n_kv, \
-                       head_dim, page_size, n_pages, scale, cut, w, stream)
+    weigh_float<T, DP>((const T*)q, q_row_stride, (const T*)k_pages, block_table, table_width, cu_q, kv_len, stats, parts, n_direct, n_seqs, max_kv, n_heads, \
+                       n_kv, head_dim, page_size, n_pages, scale, cut, w, stream)
 #define OF_TYPE(T) (head_dim <= 32 ? OF_SIZE(T, 32) : head_dim <= 64 ? OF_SIZE(T, 64) : head_dim <= 128 ? OF_SIZE(T, 128) : OF_SIZE(T, 256))
     return dtype == SIA_F32 ? OF_TYPE(float) : OF_TYPE(bf16_t);
 #undef OF_TYPE

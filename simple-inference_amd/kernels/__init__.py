@@ -109,7 +109,7 @@ _SIGNATURES = {
                           _c_ptr, _c_float, _c_int, _c_ptr],
     "sia_attention_max_head_dim": [],
     "sia_attention_generic_max_head_dim": [],
-    "sia_attention_weighed_workspace": [_c_int] * 7,
+    "sia_attention_weighed_workspace": [_c_int] * 8,
     "sia_attention_weighed": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int,
                               _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_ptr, _c_ptr, _c_int,
                               _c_int, _c_int, _c_ptr],
@@ -2107,7 +2107,7 @@ class HipKernels:
                 places, stream), "attn_weighed")
             return out
         q_bound = int(ctx.max_q_len)
-        ws = weights.new_empty((self.core.sia_attention_weighed_workspace(n, q_bound, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim),))
+        ws = weights.new_empty((self.core.sia_attention_weighed_workspace(n, n_single, q_bound, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim),))
         self._check(self.core.sia_attention_weighed(
             *given, ctx.seq_of_token.data_ptr(), ctx.positions.data_ptr(), ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), out.data_ptr(),
             ws.data_ptr(), n, n_single, ctx.n_seqs, q_bound, max_kv, n_heads, n_kv_heads, head_dim, value_dim, page, cache.k_pages.shape[0],

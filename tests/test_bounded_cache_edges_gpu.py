@@ -63,7 +63,7 @@ def grown_by(call):
     return torch.cuda.max_memory_allocated() - there
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16])
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_short_rows_beside_a_long_run(hip, dtype):
     """Single tokens over some tens of keys, one of them over nothing but itself, beside a portion over thousands: right, and with workspaces for
     the keys and rows that there are."""
@@ -79,3 +79,31 @@ def test_short_rows_beside_a_long_run(hip, dtype):
     out = hip.weighed_attention(qkv, heads, kv, dim, 0.125, ctx, cache)
     ctx.max_single_kv_len = 0                    # not known: the step's own bound
     assert torch.equal(hip.weighed_attention(qkv, heads, kv, dim, 0.125, ctx, cache), out)
+
+
+def test_a_group_of_more_heads_than_a_chunk_has_rows(hip):
+    """Float heads, 65 and 70 of them a key/value head: single tokens have chunks too."""
+    for heads, kv in ((65, 1), (140, 2)):
+        ctx, cache = Ctx([1, 1, 20], [300, 7, 90]), Cache([300, 7, 90], kv, 16, 32, torch.float32)
+        check_weighed(hip, ctx, cache, rnd(ctx.n_tokens, heads * 32, seed=8), heads, 32 ** -0.5)
+
+
+def test_many_short_rows_in_float32(hip):
+    """More pieces of work than a row of the grid has: 5,000 single tokens, and a run, under a bound of 2,000 keys."""
+    q_lens, lens = [1] * 5000 + [50], [1 + i % 37 for i in range(5000)] + [2000]
+    ctx, cache = Ctx(q_lens, lens), Cache(lens, 1, 16, 16, torch.float32)
+    qkv = rnd(ctx.n_tokens, 16, seed=8)
+    before = cache.weights.clone()
+    out = hip.weighed_attention(qkv, 1, 1, 16, 0.25, ctx, cache)
+    got = cache.weights.clone()
+    for s in (0, 1, 36, 37, 2500, 4094, 4095, 4096, 4999, 5000):      # alone they have the same bits, or a run's sums up to their order
+        alone = Cache([lens[s]], 1, 16, 16, torch.float32)
+        alone.k_pages, alone.v_pages, alone.block_table = cache.k_pages, cache.v_pages, cache.block_table[s:s + 1].contiguous()
+        alone.weights = before[s:s + 1].clone()
+        rows = slice(int(ctx.cu_q[s]), int(ctx.cu_q[s + 1]))
+        one = check_weighed(hip, Ctx([q_lens[s]], [lens[s]], [0]), alone, qkv[rows].contiguous(), 1, 0.25, poison=False)
+        assert torch.equal(one, out[rows])
+        if q_lens[s] == 1:
+            assert torch.equal(alone.weights[0], got[s])
+        else:
+            torch.testing.assert_close(alone.weights[0], got[s], rtol=50 * 2 * STEP32, atol=0)
