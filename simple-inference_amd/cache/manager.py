@@ -28,6 +28,10 @@ Beside the pages there are *slots*: one row of fixed size per running request
 and per stateful run of a layer, set to the state's initial value when a request gets its slot.  The
 architecture served here has no such state; the slots still exist, every request
 holds one, and the step function hands the slot ids to every mixer.
+
+For attention that adds up the weight every cached key gets (``HipKernels.weighed_attention``) the manager keeps the sums
+(``keep_weights``): a row per slot, in which the places that a step writes begin at zero in that step, and the places of adopted
+pages, which no step of the request writes, at its admission.
 """
 
 from __future__ import annotations
@@ -64,7 +68,7 @@ class PagedGroup:
         # numbers come from one counter, so an id that is admitted again never meets a number it had before
         self.versions: Dict[int, int] = {}
         self._version = 0
-        self.k = self.v = None
+        self.k = self.v = self.weights = None
         if allocate_storage:
             shape_k = (slabs, num_pages + 1, need.num_kv_heads, page_size, need.head_dim)
             shape_v = (slabs, num_pages + 1, need.num_kv_heads, need.value_dim, page_size)
@@ -171,12 +175,24 @@ class CacheManager:
                  dtype: torch.dtype, device, allocate_storage: bool = True):
         self.layout = layout
         self.page_size = page_size
+        self.device = device
         self.groups = [
             PagedGroup(need, slabs, page_size, num_pages, dtype, device, allocate_storage)
             for need, slabs in zip(layout.kv_groups, layout.kv_slabs)
         ]
         self.slots = StateSlots(layout.states, max_running, device, allocate_storage)
         self.lengths: Dict[int, int] = {}
+
+    def keep_weights(self, places: int) -> None:
+        """From now on the layers' caches have sums of attention weight (``LayerCache.weights``), float32 ``[slots + 1, kv_heads,
+        places]`` for each, zeros at first; no request is longer than ``places``.  To be asked for while no request is admitted."""
+        if places <= 0:
+            raise ValueError(f"places must be positive, got {places}")
+        if self.lengths:
+            raise ValueError("the sums of requests that run already would be missing")
+        for g in self.groups:
+            g.weights = torch.zeros(g.slabs, self.slots.max_running + 1, g.need.num_kv_heads, places, dtype=torch.float32,
+                                    device=self.device)
 
     # -- admission ---------------------------------------------------------
     def can_admit(self, total_tokens: Optional[int], max_chunk: int = 1, shared_pages: int = 0) -> bool:
@@ -212,6 +228,8 @@ class CacheManager:
                 g.pool.adopt(req, page)
                 g.tables[req].append(page)
                 g._touch(req)
+            if shared and g.weights is not None:
+                g.weights[:, slot, :, :len(shared) * self.page_size].zero_()
         self.lengths[req] = len(shared) * self.page_size
         return slot
 
@@ -280,6 +298,8 @@ class CacheManager:
                 g, slab = kv
                 grp = self.groups[g]
                 c.k_pages, c.v_pages = grp.k[slab], grp.v[slab]
+                if grp.weights is not None:
+                    c.weights = grp.weights[slab]
                 c.block_table = block_tables[g]
                 c.page_size = grp.page_size
             si = self.layout.run_state[e]

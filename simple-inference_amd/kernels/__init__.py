@@ -2066,7 +2066,8 @@ class HipKernels:
         """``paged_attention`` (without window, blocks and cap) that also adds up how much weight every cached key gets:
         ``cache.weights[slot, g, place]`` (float32 ``[slots, n_kv_heads, places]``; a sequence's row is ``ctx.state_slots[s]``, each
         sequence with a row of its own) grows by the sum, over the sequence's tokens of this step and the query heads of ``g``, of
-        their softmax weights.  The sums of the places that the step itself has written begin at zero.  ``sinks`` take their share
+        their softmax weights.  The sums of the places that the step itself has written begin at zero; those of places
+        that no step of the request writes (adopted pages) have to hold zeros when it begins, as ``CacheManager.keep_weights`` sees to.  ``sinks`` take their share
         of a row's weight and have no place.  A row of a sequence without places is zeros.  Prompts, portions and single tokens, mixed as
         ``ctx`` says."""
         self._want(qkv, "qkv")

@@ -107,3 +107,43 @@ def test_many_short_rows_in_float32(hip):
             assert torch.equal(alone.weights[0], got[s])
         else:
             torch.testing.assert_close(alone.weights[0], got[s], rtol=50 * 2 * STEP32, atol=0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_request_with_an_adopted_prefix(hip, dtype):
+    """Its sums hold what its own tokens gave the adopted places, and nothing of whoever had its slot before; once it is the pages' only holder,
+    eviction goes by them."""
+    from simple_inference_amd.cache import CacheManager
+    from simple_inference_amd.parts.model import CacheLayout
+    from simple_inference_amd.parts.plan import PagedKVNeed
+    heads, kv, dim, page = 4, 2, 64, 16
+    plan = CacheLayout([PagedKVNeed(kv, dim, None)], [1], [(0, 0)], [], [None])
+    books = CacheManager(plan, page_size=page, num_pages=24, max_running=3, dtype=dtype, device=DEV)
+    books.keep_weights(160)
+    cos, sin = angles(200, 32)
+
+    def layer_of(req):
+        return books.layer_caches([torch.tensor([books.table(0, req)], dtype=torch.int32, device=DEV)])[0]
+
+    def step(req, n):
+        length = books.extend(req, n) + n
+        ctx, layer = Ctx([n], [length], [books.slot(req)]), layer_of(req)
+        qkv = rnd(n, (heads + 2 * kv) * dim, dtype=dtype, seed=100 * req + length)
+        hip.rope_axes_kv_write(qkv, heads, kv, dim, (32,), cos, sin, ctx.positions[None].contiguous(), ctx, layer)
+        view = Cache([length], kv, page, dim, dtype)      # for its way of looking at pages
+        view.k_pages, view.v_pages, view.block_table, view.weights = layer.k_pages, layer.v_pages, layer.block_table, layer.weights
+        check_weighed(hip, ctx, view, qkv, heads, 0.125, poison=False)
+        return ctx, view
+
+    books.admit(1)
+    step(1, 70)
+    books.groups[0].weights[:, 1:] = math.nan             # what others left in the other rows
+    slot = books.admit(2, shared_pages=books.table(0, 1)[:4])
+    ctx, view = step(2, 30)
+    got = view.weights[slot, :, :94].double()
+    assert torch.allclose(got.sum(-1), torch.full((kv,), 30.0 * heads / kv, dtype=torch.float64, device=DEV), rtol=1e-4)
+    books.release(1)
+    assert books.owns_pages(2)
+    check_evict(hip, ctx, view, 40, 2, 8)
+    books.shrink(2, 40)
+    books.check()
