@@ -108,6 +108,14 @@ class PagePool:
             acct.promised += 1
             self._promised += 1
 
+    def limit_promise(self, owner: int, promise: int) -> None:
+        """What the owner may still take for certain is at most ``promise`` pages from now on."""
+        if promise < 0:
+            raise ValueError(f"a promise cannot be negative ({promise})")
+        acct = self._account(owner)
+        self._promised -= max(0, acct.promised - promise)
+        acct.promised = min(acct.promised, promise)
+
     def pin(self, page: int) -> None:
         """One more holder of a page in use, outside every account."""
         self._hold_once_more(page, "pinned")

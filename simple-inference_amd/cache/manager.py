@@ -111,14 +111,17 @@ class PagedGroup:
             table.extend(self.pool.take_many(req, more))
             self._touch(req)
 
-    def shrink(self, req: int, tokens: int) -> None:
-        """Gives back the pages behind place ``tokens - 1``; the request may take as many again."""
+    def shrink(self, req: int, tokens: int, most: Optional[int] = None) -> None:
+        """Gives back the pages behind place ``tokens - 1``; the request may take as many again, or with ``most`` as many as that
+        many places take."""
         table, keep = self.tables[req], pages_for(tokens, self.page_size)
         if len(table) > keep:
             for page in table[keep:]:
                 self.pool.drop(req, page, restore_promise=True)
             del table[keep:]
             self._touch(req)
+        if most is not None:
+            self.pool.limit_promise(req, max(0, pages_for(most, self.page_size) - len(table)))
 
     def _touch(self, req: int) -> None:
         self._version += 1
@@ -254,18 +257,25 @@ class CacheManager:
         moves rows within them, asks for."""
         return all(g.pool.holders(p) == 1 for g in self.groups for p in g.pool.pages(req))
 
-    def shrink(self, req: int, tokens: int) -> None:
+    def shrink(self, req: int, tokens: int, most: Optional[int] = None) -> None:
         """After an eviction (``HipKernels.evict_cache`` for every layer) that left the request ``tokens`` places: its next token
-        goes to place ``tokens``, and the pages behind the last place go back to the pool, promised to the request.  From
-        then on a token's place is not its position any more, so there are neither windows nor blocks of positions."""
+        goes to place ``tokens``, and the pages behind the last place go back to the pool.  From
+        then on a token's place is not its position any more, so there are neither windows nor blocks of positions.
+
+        The pages that go back are promised to the request, which may grow to any length again: nobody else is admitted by them.
+        ``most`` says that it will not, because it is cut back in time: of what it was promised it keeps what ``most`` places (its budget
+        and a step's tokens, say) take, and the rest is anybody's.  A request whose bound is known from the start is admitted with it
+        (``total_tokens``) and never holds more."""
         if not 0 < tokens <= self.lengths[req]:
             raise ValueError(f"request {req} holds {self.lengths[req]} tokens and cannot keep {tokens}")
+        if most is not None and most < tokens:
+            raise ValueError(f"request {req} keeps {tokens} tokens, more than the most of {most} places")
         if any(g.need.span is not None for g in self.groups):
             raise ValueError("a cache with a window or blocks knows its keys by their positions")
         if not self.owns_pages(req):
             raise ValueError(f"request {req} shares pages")
         for g in self.groups:
-            g.shrink(req, tokens)
+            g.shrink(req, tokens, most)
         self.lengths[req] = tokens
 
     def release(self, req: int) -> None:
