@@ -185,6 +185,7 @@ class CacheManager:
         ]
         self.slots = StateSlots(layout.states, max_running, device, allocate_storage)
         self.lengths: Dict[int, int] = {}
+        self._shrunk: set = set()      # requests whose places are not their tokens' positions any more
 
     def keep_weights(self, places: int) -> None:
         """From now on the layers' caches have sums of attention weight (``LayerCache.weights``), float32 ``[slots + 1, kv_heads,
@@ -277,12 +278,19 @@ class CacheManager:
         for g in self.groups:
             g.shrink(req, tokens, most)
         self.lengths[req] = tokens
+        self._shrunk.add(req)
+
+    def has_shrunk(self, req: int) -> bool:
+        """Whether tokens of the request have been dropped: place ``i`` then holds any of its tokens, so that its pages are no prefix
+        of its tokens (to be kept for others), and a step's rotation needs positions of its own."""
+        return req in self._shrunk
 
     def release(self, req: int) -> None:
         for g in self.groups:
             g.release(req)
         self.slots.give_back(req)
         self.lengths.pop(req, None)
+        self._shrunk.discard(req)
 
     def reset(self) -> None:
         for req in list(self.lengths):

@@ -51,6 +51,7 @@ class PrefixCache:
             raise ValueError(f"max_pages must be positive, got {max_pages}")
         if len(cache.groups) != 1 or cache.groups[0].need.span is not None or cache.layout.states:
             raise ValueError("prefix reuse needs one cache group without a window and no per-request state")
+        self.cache = cache
         self.pool = cache.groups[0].pool
         self.page_size = cache.page_size
         self.capacity = max_pages
@@ -146,6 +147,12 @@ class PrefixCache:
             self._hits += 1
             self._reused += self.page_size * len(pages)
         return pages
+
+    def insert_pages_of(self, req: int, tokens) -> None:
+        """``insert`` of an admitted request's pages, whose first tokens these are; nothing of one that has dropped tokens, whose
+        pages hold others of its tokens, in another order."""
+        if not self.cache.has_shrunk(req):
+            self.insert(tokens, self.cache.table(0, req))
 
     def insert(self, tokens, page_table: List[int]) -> None:
         """Keeps every complete page of ``tokens`` whose keys and values are written; ``page_table[i]`` is the

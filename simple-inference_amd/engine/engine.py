@@ -228,7 +228,7 @@ class Engine:
             for req, _ in plan:
                 if req.state is RequestState.PREFILL:
                     # pages a prompt has filled so far can be shared from the next step on
-                    self.prefix_cache.insert(req.prompt_tokens[:req.num_computed], self.cache.table(0, req.id))
+                    self.prefix_cache.insert_pages_of(req.id, req.prompt_tokens[:req.num_computed])
         if not emitters:
             return [], None
         with self.ranges("engine.sample"):

@@ -78,6 +78,9 @@ class StepRunner:
                 raise ValueError(f"request {e.req} brings no tokens")
             if e.req not in self.cache.lengths:
                 raise KeyError(f"request {e.req} is not admitted to the cache")
+            if not e.extra and self.cache.has_shrunk(e.req):
+                raise ValueError(f"request {e.req} has dropped tokens, so its places are not its positions: its tokens need positions of "
+                                 f"their own (StepEntry.extra)")
             if self.cache.lengths[e.req] + len(e.tokens) > self.max_positions:
                 raise ValueError(
                     f"request {e.req} would reach position {self.cache.lengths[e.req] + len(e.tokens)}, "
