@@ -15,10 +15,10 @@ from ..weights.loader import load_weights, target_dtype
 from ..weights.random_init import random_tensors
 
 
-def default_kernels():
-    """The compiled HIP kernel library; raises if it cannot be had."""
+def default_kernels(device="cuda:0"):
+    """The compiled HIP kernel library, for work on that device; raises if it cannot be had."""
     from ..kernels import HipKernels
-    return HipKernels()
+    return HipKernels(device if torch.device(device).type == "cuda" else "cuda:0")
 
 
 def build_model(config_dict: Mapping, engine_cfg: EngineConfig, kernels):
@@ -67,7 +67,7 @@ def describe(model, model_cfg, engine_cfg: EngineConfig) -> str:
 
 
 def model_from_folder(folder, engine_cfg: EngineConfig, kernels=None):
-    kernels = kernels if kernels is not None else default_kernels()
+    kernels = kernels if kernels is not None else default_kernels(engine_cfg.device)
     model, model_cfg = build_model(read_config_json(folder), engine_cfg, kernels)
     count_parameters(model, model_cfg)
     tensors = load_weights(folder, model.expected_tensors(), engine_cfg.device, engine_cfg.torch_dtype,
@@ -81,7 +81,7 @@ def model_from_random(config_dict: Mapping, seed: int, engine_cfg: EngineConfig,
                       generate_on_device: bool = False):
     """Random weights without a folder.  Values are drawn in ``storage`` dtype first, so
     that a bfloat16 and a float32 engine built from the same seed hold the same numbers."""
-    kernels = kernels if kernels is not None else default_kernels()
+    kernels = kernels if kernels is not None else default_kernels(engine_cfg.device)
     model, model_cfg = build_model(config_dict, engine_cfg, kernels)
     expected = model.expected_tensors()
     device = engine_cfg.device if generate_on_device else "cpu"

@@ -84,7 +84,7 @@ class Engine:
     @classmethod
     def from_folder(cls, folder, engine_cfg: Optional[EngineConfig] = None, kernels=None) -> "Engine":
         engine_cfg = engine_cfg or EngineConfig()
-        kernels = kernels if kernels is not None else default_kernels()
+        kernels = kernels if kernels is not None else default_kernels(engine_cfg.device)
         model, model_cfg = model_from_folder(folder, engine_cfg, kernels)
         engine = cls(model, model_cfg, engine_cfg, kernels)
         engine.model_folder = folder
@@ -94,7 +94,7 @@ class Engine:
     def from_random(cls, config_dict, seed: int = 0, engine_cfg: Optional[EngineConfig] = None, kernels=None,
                     **random_options) -> "Engine":
         engine_cfg = engine_cfg or EngineConfig()
-        kernels = kernels if kernels is not None else default_kernels()
+        kernels = kernels if kernels is not None else default_kernels(engine_cfg.device)
         model, model_cfg = model_from_random(config_dict, seed, engine_cfg, kernels, **random_options)
         return cls(model, model_cfg, engine_cfg, kernels)
 

@@ -349,7 +349,8 @@ class HipKernels:
         # the short way to the current stream's handle, where this torch has it (a few microseconds less a launch)
         self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self._current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-        self._device_index = torch.device(device).index or 0
+        index = self.device.index
+        self._device_index = torch.cuda.current_device() if index is None else index
         self._axes_known: Dict[tuple, tuple] = {}       # what ``rope_axes_kv_write`` makes of its plain arguments
         self.use_mfma_attention = True   # tests switch it off to reach the plain kernel in bfloat16
         self.use_skinny_gemm = True      # few-row bfloat16 products by this package's kernel, not the library
@@ -447,9 +448,10 @@ class HipKernels:
                 raise KernelError(f"{what}: the kernel refused its arguments (sizes or types it does not take)")
             raise KernelError(f"{what}: HIP error {code}")
 
-    def _want(self, t: torch.Tensor, what: str, dtype=None, shape=None):
-        if t.get_device() != self._device_index:
-            raise KernelError(f"{what} must be on the GPU (cuda:{self._device_index}), is on {t.device}")
+    def _want(self, t: torch.Tensor, what: str, dtype=None, shape=None, here=False):
+        """``here``: on the kernels' own device (goes with ``_stream_here``), not on any GPU."""
+        if t.get_device() != self._device_index if here else not t.is_cuda:
+            raise KernelError(f"{what} must be on the GPU{f' (cuda:{self._device_index})' if here else ''}, is on {t.device}")
         if not t.is_contiguous():
             raise KernelError(f"{what} must be contiguous")
         if dtype is not None and t.dtype != dtype:
@@ -1719,7 +1721,7 @@ class HipKernels:
         ``j mod axes`` while that has fewer than its section, else to axis 0).  ``pairing``: ``"half"`` (elements ``i`` and ``i +
         rotary_dim / 2``) or ``"interleaved"`` (neighbours).  ``cos``, ``sin``: float32 tables ``[positions, pairs]``; a position
         outside them is taken at the nearest row."""
-        self._want(qkv, "qkv")
+        self._want(qkv, "qkv", here=True)
         if qkv.dtype not in _DT or qkv.dim() != 2:
             raise KernelError(f"qkv must be a float32 or bfloat16 matrix, is {qkv.dtype} {tuple(qkv.shape)}")
         n, width = qkv.shape
@@ -1732,16 +1734,16 @@ class HipKernels:
         if known is None:
             known = self._axes_known[key] = self._axes(*key)
         counts, axes, half, cycled, neighbours = known
-        self._want(cos, "cos table", torch.float32)
-        self._want(sin, "sin table", torch.float32)
+        self._want(cos, "cos table", torch.float32, here=True)
+        self._want(sin, "sin table", torch.float32, here=True)
         if cos.dim() != 2 or cos.shape[0] < 1 or cos.shape[1] != half or sin.shape != cos.shape:
             raise KernelError(f"cos and sin tables {tuple(cos.shape)} and {tuple(sin.shape)} do not hold {half} pairs")
-        self._want(rotary_positions, "rotary positions", torch.int32, (axes, n))
+        self._want(rotary_positions, "rotary positions", torch.int32, (axes, n), here=True)
         k = v = table = None
         page_size = pages = table_width = 0
         if n_kv_written:
             k_pages, v_pages, block_table, page_size = cache.k_pages, cache.v_pages, cache.block_table, cache.page_size
-            self._check_pages(k_pages, v_pages, block_table, page_size, n_kv_written, head_dim, qkv.dtype, ctx)
+            self._check_pages(k_pages, v_pages, block_table, page_size, n_kv_written, head_dim, qkv.dtype, ctx, here=True)
             k, v, table = k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr()
             pages, table_width = k_pages.shape[0], block_table.shape[1]
         self._check(self.core.sia_rope_axes_kv_write(
@@ -1978,16 +1980,16 @@ class HipKernels:
             _ptr(convolved), _DT[proj.dtype], self._stream()), "row_prepare")
         return q
 
-    def _check_pages(self, k_pages, v_pages, table, page_size, n_kv, head_dim, dtype, ctx, value_dim=None):
+    def _check_pages(self, k_pages, v_pages, table, page_size, n_kv, head_dim, dtype, ctx, value_dim=None, here=False):
         value_dim = value_dim or head_dim
-        self._want(k_pages, "key pages", dtype)
-        self._want(v_pages, "value pages", dtype)
+        self._want(k_pages, "key pages", dtype, here=here)
+        self._want(v_pages, "value pages", dtype, here=here)
         pages = k_pages.shape[0]
         if k_pages.shape != (pages, n_kv, page_size, head_dim):
             raise KernelError(f"key pages {tuple(k_pages.shape)} are not [pages, {n_kv}, {page_size}, {head_dim}]")
         if v_pages.shape != (pages, n_kv, value_dim, page_size):
             raise KernelError(f"value pages {tuple(v_pages.shape)} are not [pages, {n_kv}, {value_dim}, {page_size}]")
-        self._want(table, "block table", torch.int32)
+        self._want(table, "block table", torch.int32, here=here)
         if table.dim() != 2 or table.shape[0] != ctx.n_seqs or table.shape[1] * page_size < ctx.max_kv_len:
             raise KernelError(f"block table {tuple(table.shape)} does not cover {ctx.n_seqs} sequences of up to "
                               f"{ctx.max_kv_len} positions with pages of {page_size}")
@@ -2055,11 +2057,11 @@ class HipKernels:
         weights, most = cache.weights, int(max(ctx.kv_bound or 0, ctx.max_kv_len))
         if weights is None:
             raise KernelError("the cache keeps no weights (LayerCache.weights)")
-        self._want(weights, "weights", torch.float32)
+        self._want(weights, "weights", torch.float32, here=True)
         if weights.dim() != 3 or weights.shape[0] < 1 or weights.shape[1] != n_kv or weights.shape[2] < max(1, most):
             raise KernelError(f"weights {tuple(weights.shape)} are not [slots, {n_kv}, places] with room for {most} places")
         for t, what in ((ctx.state_slots, "state slots"), (ctx.kv_len, "lengths")):
-            self._want(t, what, torch.int32, (ctx.n_seqs,))
+            self._want(t, what, torch.int32, (ctx.n_seqs,), here=True)
         return weights, most
 
     def weighed_attention(self, qkv, n_heads, n_kv_heads, head_dim, scale, ctx, cache, value_dim=None, sinks=None):
@@ -2070,7 +2072,7 @@ class HipKernels:
         that no step of the request writes (adopted pages) have to hold zeros when it begins, as ``CacheManager.keep_weights`` sees to.  ``sinks`` take their share
         of a row's weight and have no place.  A row of a sequence without places is zeros.  Prompts, portions and single tokens, mixed as
         ``ctx`` says."""
-        self._want(qkv, "qkv")
+        self._want(qkv, "qkv", here=True)
         if qkv.dtype not in _DT or qkv.dim() != 2:
             raise KernelError(f"qkv must be a float32 or bfloat16 matrix, is {qkv.dtype} {tuple(qkv.shape)}")
         n, width = qkv.shape
@@ -2083,9 +2085,9 @@ class HipKernels:
         if width < n_heads * head_dim or n != ctx.n_tokens:
             raise KernelError(f"qkv {tuple(qkv.shape)} does not hold {ctx.n_tokens} rows of {n_heads} heads of {head_dim}")
         self._check_pages(cache.k_pages, cache.v_pages, cache.block_table, cache.page_size, n_kv_heads, head_dim, qkv.dtype, ctx,
-                          value_dim)
+                          value_dim, here=True)
         if sinks is not None:
-            self._want(sinks, "sinks", torch.float32, (n_heads,))
+            self._want(sinks, "sinks", torch.float32, (n_heads,), here=True)
         weights, max_kv = self._check_weights(cache, ctx, n_kv_heads)
         out = qkv.new_empty((n, n_heads * value_dim))
         if not n:
@@ -2132,7 +2134,7 @@ class HipKernels:
         if k_pages is None or k_pages.dim() != 4 or v_pages is None or v_pages.dim() != 4 or k_pages.dtype not in _DT:
             raise KernelError("the cache has no float32 or bfloat16 pages of keys and values")
         n_kv, head_dim, value_dim = k_pages.shape[1], k_pages.shape[3], v_pages.shape[2]
-        self._check_pages(k_pages, v_pages, table, cache.page_size, n_kv, head_dim, k_pages.dtype, ctx, value_dim)
+        self._check_pages(k_pages, v_pages, table, cache.page_size, n_kv, head_dim, k_pages.dtype, ctx, value_dim, here=True)
         weights, max_kv = self._check_weights(cache, ctx, n_kv)
         if table.shape[1] * cache.page_size < max_kv:
             raise KernelError(f"block table {tuple(table.shape)} does not cover {max_kv} places with pages of {cache.page_size}")

@@ -33,7 +33,7 @@ class TraceReplayer:
         self.engine_cfg = EngineConfig(
             device=device, dtype=dtype, block_size=page, num_kv_blocks=num_pages, max_running=max_live,
             max_seq_len=min(max_pos, max(max_tokens, page)))
-        self.kernels = kernels if kernels is not None else default_kernels()
+        self.kernels = kernels if kernels is not None else default_kernels(device)
         self.architecture = architecture_name(cfg)
         self.model, self.model_cfg = model_from_folder(model_folder, self.engine_cfg, self.kernels)
         self.cache = CacheManager(
