@@ -459,6 +459,11 @@ class HipKernels:
         if shape is not None and t.shape != tuple(shape):
             raise KernelError(f"{what} must have shape {tuple(shape)}, has {tuple(t.shape)}")
 
+    def _want_ints(self, t: torch.Tensor, what: str, n: int):
+        """What the kernels read of a step's context: ``n`` int32 numbers on their device."""
+        if t.get_device() != self._device_index or t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
+            self._want(t, what, torch.int32, (n,), here=True)
+
     # -- measurement -----------------------------------------------------------
     def measured_read_bandwidth(self, megabytes: int = 2048, repeats: int = 5) -> float:
         """GB/s that a plain streaming read of a buffer far larger than the caches reaches on this card (the best
@@ -1746,6 +1751,8 @@ class HipKernels:
             self._check_pages(k_pages, v_pages, block_table, page_size, n_kv_written, head_dim, qkv.dtype, ctx, here=True)
             k, v, table = k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr()
             pages, table_width = k_pages.shape[0], block_table.shape[1]
+            self._want_ints(ctx.positions, "positions", n)
+            self._want_ints(ctx.seq_of_token, "sequences of tokens", n)
         self._check(self.core.sia_rope_axes_kv_write(
             qkv.data_ptr(), width, cos.data_ptr(), sin.data_ptr(), cos.shape[0], rotary_positions.data_ptr(), counts, axes, cycled,
             ctx.positions.data_ptr(), ctx.seq_of_token.data_ptr(), table, table_width, k, v, pages, n, n_heads, n_kv_written, head_dim,
@@ -2060,8 +2067,8 @@ class HipKernels:
         self._want(weights, "weights", torch.float32, here=True)
         if weights.dim() != 3 or weights.shape[0] < 1 or weights.shape[1] != n_kv or weights.shape[2] < max(1, most):
             raise KernelError(f"weights {tuple(weights.shape)} are not [slots, {n_kv}, places] with room for {most} places")
-        for t, what in ((ctx.state_slots, "state slots"), (ctx.kv_len, "lengths")):
-            self._want(t, what, torch.int32, (ctx.n_seqs,), here=True)
+        self._want_ints(ctx.state_slots, "state slots", ctx.n_seqs)
+        self._want_ints(ctx.kv_len, "lengths", ctx.n_seqs)
         return weights, most
 
     def weighed_attention(self, qkv, n_heads, n_kv_heads, head_dim, scale, ctx, cache, value_dim=None, sinks=None):
@@ -2089,6 +2096,9 @@ class HipKernels:
         if sinks is not None:
             self._want(sinks, "sinks", torch.float32, (n_heads,), here=True)
         weights, max_kv = self._check_weights(cache, ctx, n_kv_heads)
+        self._want_ints(ctx.cu_q, "first tokens", ctx.n_seqs + 1)
+        if not 0 <= ctx.n_decode_seqs <= min(ctx.n_seqs, n):
+            raise KernelError(f"{ctx.n_decode_seqs} sequences of a token each are not in a step of {ctx.n_seqs} sequences and {n} tokens")
         out = qkv.new_empty((n, n_heads * value_dim))
         if not n:
             return out
@@ -2110,6 +2120,8 @@ class HipKernels:
                 places, stream), "attn_weighed")
             return out
         q_bound = int(ctx.max_q_len)
+        self._want_ints(ctx.positions, "positions", n)
+        self._want_ints(ctx.seq_of_token, "sequences of tokens", n)
         ws = weights.new_empty((self.core.sia_attention_weighed_workspace(n, n_single, q_bound, ctx.n_seqs, max_kv, n_heads, n_kv_heads, head_dim),))
         self._check(self.core.sia_attention_weighed(
             *given, ctx.seq_of_token.data_ptr(), ctx.positions.data_ptr(), ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), out.data_ptr(),

@@ -95,6 +95,40 @@ def test_other_kernels_take_what_is_on_a_gpu():
             k._want(bad, "rows", torch.float32, (4, 8))
 
 
+READ = {"rotate": ["positions", "seq_of_token"], "attend": ["positions", "seq_of_token", "cu_q", "kv_len", "state_slots"], "evict": ["kv_len", "state_slots"]}
+
+
+@pytest.mark.parametrize("name,field", [(name, field) for name in OPERATORS for field in READ[name]])
+def test_what_the_kernels_read_of_a_context_is_checked(name, field):
+    for change in (lambda t: on(t.long()), lambda t: on(t[:-1].contiguous()), lambda t: on(torch.cat([t, t])), lambda t: on(t.repeat_interleave(2)[::2]),
+                   lambda t: on(t[None]), lambda t: on(t.float()), lambda t: t.as_subclass(torch.Tensor), lambda t: on(t, OnSecondGpu)):
+        k, (ctx, _, calls) = kernels(), a_step()
+        own, changed = getattr(ctx, field), change(getattr(ctx, field))
+        if changed.is_contiguous() and changed.shape == own.shape and changed.dtype == own.dtype and type(changed) is OnGpu:
+            continue      # (one number in every other place is one number)
+        setattr(ctx, field, changed)
+        with pytest.raises(KernelError):
+            calls[name](k)
+        assert ENTRIES[name] not in k.core.calls
+
+
+@pytest.mark.parametrize("n_decode", [-1, 2])
+def test_single_tokens_that_a_step_has_not(n_decode):
+    k, (ctx, _, calls) = kernels(), a_step()
+    ctx.n_decode_seqs = n_decode
+    with pytest.raises(KernelError):
+        calls["attend"](k)
+    assert ENTRIES["attend"] not in k.core.calls
+
+
+def test_a_rotation_without_pages_reads_no_places():
+    k, (ctx, _, _) = kernels(), a_step()
+    ctx.positions = ctx.seq_of_token = torch.zeros(0)
+    qkv, table, where = on(torch.zeros(3, 4 * 64)), on(torch.zeros(8, 32)), on(torch.zeros(2, 3, dtype=torch.int32))
+    k.rope_axes_kv_write(qkv, 4, 0, 64, (16, 16), table, table, where, ctx, None)
+    assert k.core.calls[-1] == "sia_rope_axes_kv_write"
+
+
 class Built(Exception):
     pass
 
