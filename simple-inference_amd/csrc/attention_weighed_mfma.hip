@@ -390,8 +390,6 @@ static int shares_of(int group) {
     return group;
 }
 
-SIA_EXPORT int sia_attn_weighed_max_group() { return JOIN_MOST_HEADS; }
-
 // Floats of the single tokens' workspace: scores, and the splits' states.
 static long long single_floats(int n_single, int n_heads, int max_kv) {
     return n_single <= 0 ? 0 : (long long)n_single * n_heads * (row_keys_of(max_kv) + (long long)splits_of(max_kv) * (HD + 2));

@@ -227,7 +227,6 @@ _ATTN_SIGNATURES = {
 
 # of the libraries without the forms
 _WEIGHED_SIGNATURES = {
-    "sia_attn_weighed_max_group": [],
     "sia_attn_weighed_workspace": [_c_int] * 8,
     "sia_attn_weighed": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int,
                          _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
@@ -2108,7 +2107,8 @@ class HipKernels:
         if (self.use_mfma_attention and qkv.dtype == torch.bfloat16 and head_dim % 16 == 0 and head_dim <= 256 and value_dim == head_dim
                 and page >= 8 and page & (page - 1) == 0 and width % 8 == 0 and scale > 0 and n_heads // n_kv_heads <= 256
                 and _in_pieces(qkv, cache.k_pages, cache.v_pages)):
-            # single tokens by one walk over keys and values, runs by the attention kernel and the scores once more
+            # single tokens by one walk over keys and values, runs by the attention kernel and the scores once more (256: the query heads of a
+            # key/value head whose statistics the join holds)
             lib = self._attn_lib(head_dim)
             tiles, q_bound, run_kv = self._run_tiles(lib, ctx) if n_single < ctx.n_seqs else ((0, 0, 0), 0, 0)
             if n_single:      # scores, splits and the join's grid are those of the longest single token
