@@ -147,3 +147,151 @@ def test_a_request_with_an_adopted_prefix(hip, dtype):
     check_evict(hip, ctx, view, 40, 2, 8)
     books.shrink(2, 40)
     books.check()
+
+
+def compare(got, want, bound):
+    """How many times the bound a result is off at worst."""
+    return float(((got - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [0.0, -0.11])
+def test_scales_that_are_not_positive(hip, dtype, scale):
+    """Every key alike, and the largest product the least weight: by the kernels that take any scale."""
+    lens, starts, dim = [33, 600, 300], [32, 599, 260], 64
+    ctx, cache = Ctx([1, 1, 40], lens), Cache(lens, 2, 16, dim, dtype)
+    qkv = rnd(ctx.n_tokens, 4 * dim, dtype=dtype, seed=8)
+    before = cache.weights.double()
+    out = hip.weighed_attention(qkv, 4, 2, dim, scale, ctx, cache).double().view(-1, 4, dim)
+    q, cu, half = qkv.double().view(-1, 4, dim), ctx.cu_q.tolist(), torch.finfo(dtype).eps / 2
+    for s, length in enumerate(lens):
+        k, v = cache.rows(s, length)
+        for g in range(2):
+            grown, size, rows = torch.zeros(length, dtype=torch.float64, device=DEV), 0.0, slice(cu[s], cu[s + 1])
+            for h in (2 * g, 2 * g + 1):
+                o, p, _ = attended(q[rows, h], k[g], v[g], starts[s], scale, None)
+                terms = float((q[rows, h].abs() @ k[g].abs().T).max() * abs(scale))
+                rel = 2 * (dim + 8) * terms * STEP32 + (length + 80) * STEP32 + 8 * STEP32 * (terms + 8)      # as in check_weighed
+                assert compare(out[rows, h], o, half * o.abs() + (p @ v[g].abs()) * (2 * rel + 1.01 * half) + 1e-30) <= 1
+                grown, size = grown + p.sum(0), max(size, rel)
+            want = grown + torch.where(torch.arange(length, device=DEV) < starts[s], before[s, g, :length], 0.0)
+            count = 2 * ctx.q_lens[s]
+            assert compare(cache.weights[s, g, :length].double(), want, grown * (2 * size + count * STEP32) + want * 4 * STEP32 + 1e-30) <= 1
+
+
+@pytest.mark.parametrize("q_lens,kv_lens,heads,kv,dim", [([1] * 3, [33, 1, 700], 8, 2, 128), ([1, 60, 3], [40, 60, 500], 6, 2, 64), ([1, 20], [90, 200], 4, 1, 256)])
+def test_bfloat16_without_its_matrix_cores(hip, q_lens, kv_lens, heads, kv, dim):
+    ctx, cache = Ctx(q_lens, kv_lens), Cache(kv_lens, kv, 16, dim, torch.bfloat16)
+    qkv = rnd(ctx.n_tokens, heads * dim, dtype=torch.bfloat16, seed=8)
+    hip.use_mfma_attention = False
+    try:
+        check_weighed(hip, ctx, cache, qkv, heads, dim ** -0.5)
+    finally:
+        hip.use_mfma_attention = True
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_requests_sums_from_its_first_token_on(hip, dtype):
+    """A prompt, tokens and a portion with evictions between, each operator against its definition on what the one before it left, and the sums
+    against a list per head that is kept in 64 bits and never takes a number from the kernels.  The bounds are relative to every single sum, so that
+    sums of another head, of too few heads or of none are beyond them: the list's own mistakes show it."""
+    heads, kv, dim, budget, first, last, scale = 6, 2, 64, 96, 2, 24, 0.125
+    group, sections, pages = heads // kv, (12, 10, 10), 16
+    cache = Cache([256], kv, pages, dim, dtype)
+    cache.weights.fill_(math.nan)
+    cos, sin = angles(400, 32)
+    held = [torch.zeros(2, 0, dtype=torch.float64, device=DEV) for _ in range(kv)]      # per head: sums, and how far the kernels' may be off
+    length = at = 0
+    for n in [150] + [1] * 10 + [30] + [1] * 5:
+        token = torch.arange(at, at + n, dtype=torch.int32)
+        where = torch.stack([token, token // 2, token % 7]).to(DEV)
+        at, length = at + n, length + n
+        ctx = Ctx([n], [length])
+        qkv = rnd(n, (heads + 2 * kv) * dim, dtype=dtype, seed=at)
+        turned, off = rotated(qkv, heads + kv, dim, sections, cos, sin, where, "blocks", "half")
+        off = off + (torch.finfo(dtype).eps / 2 * (turned.abs() + off) if dtype != torch.float32 else 0)
+        values = qkv[:, (heads + kv) * dim:].double().view(n, kv, dim)
+        hip.rope_axes_kv_write(qkv, heads, kv, dim, sections, cos, sin, where, ctx, cache)
+        q = qkv[:, :heads * dim].double().view(n, heads, dim)
+        k, v = cache.rows(0, length)
+        assert ((q - turned[:, :heads]).abs() <= off[:, :heads]).all()
+        assert ((k[:, length - n:].transpose(0, 1) - turned[:, heads:]).abs() <= off[:, heads:]).all()
+        assert torch.equal(v[:, length - n:].transpose(0, 1), values)
+        check_weighed(hip, ctx, cache, qkv, heads, scale)
+        got = cache.weights[0, :, :length].double()
+        for g in range(kv):
+            grown, rel = [], 0.0
+            for h in range(g * group, (g + 1) * group):
+                _, p, terms = attended(q[:, h], k[g], v[g], length - n, scale, None)
+                grown.append(p.sum(0))
+                rel = max(rel, float(2 * (dim + 8) * terms * STEP32 + (length + 80) * STEP32 + 8 * STEP32 * (terms + 8)))      # as in check_weighed
+            held[g] = torch.cat([held[g], torch.zeros(2, n, dtype=torch.float64, device=DEV)], 1)
+            short = held[g][0] + sum(grown[1:])
+            held[g][0] += sum(grown)
+            held[g][1] += sum(grown) * (2 * rel + n * group * STEP32) + held[g][0] * 4 * STEP32
+            sums, bound = held[g][0], held[g][1] + 1e-30
+            assert compare(got[g], sums, bound) <= 1
+            for wrong in (short, sums.roll(1), torch.zeros_like(sums), got[1 - g]):
+                assert compare(got[g], wrong, bound) > 1
+        if length > budget:
+            own = cache.weights[0, :, :length].tolist()
+            kept, lengths = check_evict(hip, ctx, cache, budget, first, last)
+            for g in range(kv):
+                lay = layout(own[g], length, budget, first, last)
+                assert kept[0, g].tolist() == lay
+                # what went has no more weight, by the list, than what stayed
+                gone = sorted(set(range(length)) - set(lay))
+                between = [j for j in lay if first <= j < length - last]
+                assert float((held[g][0] - held[g][1])[gone].max()) <= float((held[g][0] + held[g][1])[between].min())
+                held[g] = held[g][:, lay]
+            length = int(lengths[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_decoding_in_the_cache_managers_pages_has_the_bits_that_it_has_alone(hip, dtype):
+    """Requests that decode side by side, their caches cut to a budget and pages that one gives back taken by another: from their prompts (taken
+    one by one) on, every result, choice and sum has the bits that the request gets alone."""
+    from simple_inference_amd.cache import CacheManager
+    from simple_inference_amd.parts.model import CacheLayout
+    from simple_inference_amd.parts.plan import PagedKVNeed
+    heads, kv, dim, page, budget = 4, 2, 64, 16, 64
+    cos, sin = angles(500, 32)
+    prompts = {0: 100, 1: 30, 2: 63}
+
+    def serve(requests):
+        plan = CacheLayout([PagedKVNeed(kv, dim, None)], [1], [(0, 0)], [], [None])
+        books = CacheManager(plan, page_size=page, num_pages=24, max_running=3, dtype=dtype, device=DEV)
+        weights = torch.full((4, kv, 256), math.nan, device=DEV)
+        seen, outs = {r: 0 for r in requests}, {r: [] for r in requests}
+
+        def step(entries):
+            q_lens, lens = [n for _, n in entries], [books.extend(r, n) + n for r, n in entries]
+            ctx = Ctx(q_lens, lens, [books.slot(r) for r, _ in entries])
+            tables = [books.table(0, r) for r, _ in entries]
+            width = max(map(len, tables))
+            layer = books.layer_caches([torch.tensor([t + [-1] * (width - len(t)) for t in tables], dtype=torch.int32, device=DEV)])[0]
+            layer.weights = weights
+            rows = [rnd(n, (heads + 2 * kv) * dim, dtype=dtype, seed=1000 * r + seen[r]) for r, n in entries]
+            where = torch.cat([torch.arange(seen[r], seen[r] + n, dtype=torch.int32) for r, n in entries])
+            qkv, where = torch.cat(rows), torch.stack([where, where // 2, where // 3]).to(DEV)
+            hip.rope_axes_kv_write(qkv, heads, kv, dim, (12, 10, 10), cos, sin, where, ctx, layer)
+            out = hip.weighed_attention(qkv, heads, kv, dim, 0.125, ctx, layer)
+            kept, _ = hip.evict_cache(ctx, layer, budget, keep_first=2, keep_last=16)
+            for s, (r, n) in enumerate(entries):
+                outs[r].append((out[ctx.cu_q[s]:ctx.cu_q[s + 1]].clone(), kept[s].clone(), weights[books.slot(r), :, :min(lens[s], budget)].clone()))
+                seen[r] += n
+                if lens[s] > budget:
+                    books.shrink(r, budget)
+            books.check()
+
+        for r in requests:
+            books.admit(r)
+            step([(r, prompts[r])])
+        for _ in range(8):
+            step([(r, 1) for r in requests])
+        return outs
+
+    together = serve([0, 1, 2])
+    for r in prompts:
+        for got, want in zip(together[r], serve([r])[r]):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
