@@ -5,7 +5,8 @@
 //
 // The attention that made the output leaves lse (m + log(l) of its softmax, in units of log2: `row_stats`), so that no second pass over
 // the values is needed, only the scores again.  A place that the step itself has written begins at zero, whatever lay there.
-// All sums are float, each made by one thread in a fixed order.
+// All sums are float and have a fixed order, without atomics: over the rows of a chunk in a lane (of every 16th row, and then over 16 lanes, on the
+// matrix cores), then over the chunks of a block of keys by a kernel of their own.
 //
 // Heads of up to 256 in fours go by the float matrix cores (weigh_float_kernel), with keys as rows and queries as columns, single tokens and
 // runs alike; bfloat16 heads that the attention kernels take on the bfloat16 matrix cores by attention_weighed_mfma.hip.
@@ -78,7 +79,7 @@ __device__ __forceinline__ f32x4 load4(const bf16_t* p) {
 }
 
 // What bounds it at a few hundred tokens is the chain of loads before the first product; then the float products (157 TFLOP/s).  Three tokens over 200
-// and a prompt of 300, 32 heads of 64 on 8: 13 us beside an attention of 18.3 and a sum of the chunks of 2.6 to 3.9; the plain kernel 7,400.
+// and a prompt of 300, 32 heads of 64 on 8: 10.8 us beside an attention of 18.6 and a sum of the chunks of 2.5 to 4.0; the plain kernel 7,400.
 // DP: 32, 64, 128 or 256, the head sizes' upper bound.  The items of a key/value head are blocks keys' blocks of each of the first n_direct sequences,
 // which bring one token each (one chunk a block: straight into the weights), then most_work pieces of work of each of the others, which have parts as
 // weigh_runs_kernel's.  grid (key/value heads, items in rows of gridDim.y).

@@ -7,6 +7,12 @@
 // them into weights while it merges the splits.  A sequence of one split is finished by its one workgroup.
 // Runs of tokens (weigh_runs_kernel): the attention kernel leaves every row's statistic, and the scores are made once more, with keys as
 // rows and queries as columns: a lane holds 4 keys of 16 columns' scores, so that the sum over the queries stays in its registers to the end.
+//
+// What is rounded to fewer bits: the probabilities of the value product, to bfloat16 (off by at most 2^-8 of each), as the matrix cores take them and
+// as attention without weights has it, so that a layer gives results of the same kind whether it weighs its cache or not.  Against the definition
+// in 64 bits results are off by 0.0016 of their size for one row over 40 keys, as with probabilities in float, by 0.0014 for a prompt of 2,048, where those
+// give 0.0013, and by 0.0019 against 0.0015 at worst among other lengths: most of it is the result's own rounding.  The sums of weights are made of float exponentials of float scores; a single
+// token's scaled scores are rounded to float on their way through the workspace, where its sum of exponentials took them unrounded.
 #include "attention_tiles.h"
 #include "weighed.h"
 
@@ -204,9 +210,11 @@ constexpr int RUN_WAVES = 4, WAVE_BLOCKS = 4, WAVE_KEYS = 16 * WAVE_BLOCKS, RUN_
 // grid (key/value heads, pieces of work of a run, runs): workgroups go to the chip's dies in turn, so that with 8 key/value heads a die reads
 // one head's keys and queries.  A wave holds its 64 keys as operands; the rows come through LDS 32 at a time, two stages of it, the next tile's loads under way while one is computed.  (Read from memory as
 // operands, 16 rows of 16 bytes a lane, every lane is an access of its own to the first-level cache: four times as many, and what bound it.)
-// What bounds it: a score costs an exponential (16 cycles a wave), a multiply-add and an add (4 each), of a tile's 1,250 cycles
-// 1,016 are the vector unit's.  2,048 tokens of 24 heads of 128 on 8: 28 us, 74 before;  beside an attention
-// of 54.  Workgroups for 256, 384, 512, 768 and 1,536 of them 34.5 33.8 28.2 32.4 35.7: two are on a unit at a time, so 512 go in one round.
+// What bounds it: a score costs an exponential (16 cycles a wave), a multiply-add and an add (4 each).  2,048 tokens of 24 heads of 128 on 8: 28 us
+// (beside an attention of 54), in which 488 workgroups go in one round: 1.1 us for the piece of work, 1.9 (4.3 the longest) until the first rows and the keys
+// are there, 14 or 15 tiles of 32 rows of 1.22 us (17 in all, 22 the longest), and 0.5 for the sums.  A tile's 1.22 us are 1,460 cycles at 2.4 GHz for each of the
+// two waves of a vector unit, of which the unit's own instructions take 1,016.
+// Workgroups for 256, 384, 512, 768 and 1,536 of them 34.5 33.8 28.2 32.4 35.7: two are on a unit at a time, so 512 go in one round.
 // parts: [run][piece of work][key/value head][RUN_KEYS], or null where every block has one chunk.
 constexpr int TILE_ROWS = 32, PIECES = HD / 8, ROW_STRIDE = HD + ((HD / 16) % 2 == 0 ? 16 : 0);      // as the prefill kernel's key rows
 constexpr int RUN_THREADS = RUN_WAVES * SIA_WAVE, PER_THREAD = (TILE_ROWS * PIECES + RUN_THREADS - 1) / RUN_THREADS;

@@ -12,7 +12,7 @@
 // at or beyond the edge, their targets below it) and then the last moved up, tile after tile, in place.  Where there are few sequences, movers from
 // beyond the new length, which nothing overwrites, go to further workgroups.
 // What bounds both is latency: a chain of loads, each of whose address is the last one's result, and barriers.  us, select and move, 8 key/value heads:
-// 8 x 2,112 to 2,048 places, the last 512 kept, heads of 128: 8.2 and 12.7 (39 MB);  one of 16,384 to 4,096 17.5 and 15.7;  64 of about 700 to 509 in
+// 8 x 2,112 to 2,048 places, the last 512 kept, heads of 128: 8.2 and 12.7 (39 MB);  one of 16,384 to 4,096 17.5 and 16;  64 of about 700 to 509 in
 // float32, heads of 64: 11.6 and 49: a moved value is an element in each of its head's rows of a page, and the memory writes 64 bytes for it.
 #include "common.h"
 

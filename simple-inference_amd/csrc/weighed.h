@@ -3,8 +3,9 @@
 //
 // The rows of a key/value head are a run's (token, query head) pairs, token by token; a row sees the keys up to its token's place.  A
 // workgroup has a block of KEYS keys and a chunk of the rows that see it: min(tokens, length - first key) tokens' rows, cut into as many
-// chunks of equal size as chunk_rows asks for.  So there is no workgroup without work (half of them, if all blocks had the same chunks), and
-// they are equally long.  The chunks' sums of a block are added in order by a kernel of their own.
+// chunks of equal size as chunk_rows asks for.  So none of the workgroups of the largest run is without work (half of them would be, if all blocks had the
+// same chunks), and they are equally long; a shorter run beside it has as many, and those that it has no work for leave at once.  The chunks' sums of
+// a block are added in order by a kernel of their own.
 #pragma once
 
 #include "common.h"
