@@ -277,8 +277,9 @@ class CacheManager:
             raise ValueError(f"request {req} shares pages")
         for g in self.groups:
             g.shrink(req, tokens, most)
+        if tokens < self.lengths[req]:
+            self._shrunk.add(req)
         self.lengths[req] = tokens
-        self._shrunk.add(req)
 
     def has_shrunk(self, req: int) -> bool:
         """Whether tokens of the request have been dropped: place ``i`` then holds any of its tokens, so that its pages are no prefix

@@ -37,6 +37,17 @@ def test_pages_of_a_request_that_dropped_tokens_are_no_prefix():
     assert not cache.has_shrunk(2)
 
 
+def test_a_request_that_is_cut_back_to_what_it_has_dropped_nothing():
+    cache = manager()
+    cache.admit(1)
+    cache.extend(1, 9)
+    cache.shrink(1, 9)
+    assert not cache.has_shrunk(1)
+    cache.shrink(1, 8)
+    cache.shrink(1, 8)
+    assert cache.has_shrunk(1)
+
+
 def test_a_step_does_not_rotate_by_places(tmp_path):
     """Tokens of such a request are taken only with positions of their own; nothing is booked for those that are refused."""
     folder = write_tiny_model(tmp_path, TINIES["b"], seed=3)
